@@ -91,6 +91,33 @@ EPILOGUE = {"none": 0, "bias": 1, "relu": 2, "gelu_erf": 3, "gelu_tanh": 4, "bia
             "bias_gelu_erf": 6, "bias_gelu_tanh": 7}
 
 
+class Dropout(C.Structure):
+    _fields_ = [("probability", C.c_double), ("seed", C.c_uint64), ("sequence", C.c_uint64), ("device_sequence", C.c_void_p),
+                ("first_row", C.c_int64)]
+
+
+class DropoutMatrix(C.Structure):
+    _fields_ = [("version", C.c_uint32), ("size", C.c_size_t), ("rows", C.c_int64), ("columns", C.c_int64), ("x", C.c_void_p),
+                ("x_ld", C.c_int64), ("y", C.c_void_p), ("y_ld", C.c_int64), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32),
+                ("dropout", Dropout), ("device", C.c_int32)]
+
+
+class LayerNorm(C.Structure):
+    _fields_ = [("version", C.c_uint32), ("size", C.c_size_t), ("rows", C.c_int64), ("columns", C.c_int64), ("x", C.c_void_p),
+                ("x_ld", C.c_int64), ("gamma", C.c_void_p), ("beta", C.c_void_p), ("x_dtype", C.c_int32), ("epilogue", C.c_int32),
+                ("epsilon", C.c_float), ("device", C.c_int32), ("dropout", Dropout), ("stats", C.c_void_p), ("y", C.c_void_p),
+                ("y_ld", C.c_int64), ("dy", C.c_void_p), ("dy_ld", C.c_int64), ("dx", C.c_void_p), ("dx_ld", C.c_int64),
+                ("y_dtype", C.c_int32), ("dy_dtype", C.c_int32), ("dx_dtype", C.c_int32), ("dgamma", C.c_void_p), ("dbeta", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class Adapters(C.Structure):
+    _fields_ = [("version", C.c_uint32), ("size", C.c_size_t), ("csr", C.POINTER(QCsr)), ("adapter", C.c_void_p), ("adapters", C.c_int64),
+                ("rank", C.c_int64), ("n", C.c_int64), ("down", C.c_void_p), ("up", C.c_void_p), ("scale", C.c_void_p),
+                ("weight_dtype", C.c_int32), ("epilogue", C.c_int32), ("out", C.c_void_p), ("out_ld", C.c_int64), ("alpha", C.c_float),
+                ("beta", C.c_float), ("bias", C.c_void_p), ("row_begin", C.c_int64), ("row_end", C.c_int64), ("device", C.c_int32)]
+
+
 class BellLoweringInput(C.Structure):
     _fields_ = [("version", C.c_uint32), ("size", C.c_size_t), ("rows", C.c_uint32), ("features", C.c_uint32),
                 ("nnz", C.c_uint32), ("value_size_bytes", C.c_uint32), ("row_offsets", C.c_void_p),
@@ -258,6 +285,8 @@ EXPORTED_SYMBOLS = [
     "cb200_fleet_run_transpose", "cb200_fleet_allreduce_sum_f32",
     "cb200_host_stage_create", "cb200_host_stage_destroy", "cb200_host_stage_device_bytes", "cb200_host_forward",
     "cb200_host_encode_gene_gaps",
+    "cb200_dropout_rows", "cb200_layer_norm_forward", "cb200_layer_norm_backward_workspace", "cb200_layer_norm_backward",
+    "cb200_qcsr_adapters",
     "cb200_test_arm_wait_timeout", "cb200_test_disarm_wait_timeout",
     "cb200_session_reserve_persistent_as", "cb200_session_prepare_stream_libraries", "cb200_session_get_accounting",
     "cb200_session_graph_stable_address", "cb200_session_cache_insert", "cb200_session_cache_find",
@@ -380,6 +409,11 @@ def lib() -> C.CDLL:
         L.cb200_host_encode_gene_gaps.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32]
         L.cb200_host_forward.argtypes = [C.c_void_p, C.POINTER(QCsr), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                          C.c_float, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]
+        L.cb200_dropout_rows.argtypes = [C.POINTER(DropoutMatrix), C.c_void_p]
+        L.cb200_layer_norm_forward.argtypes = [C.POINTER(LayerNorm), C.c_void_p]
+        L.cb200_layer_norm_backward_workspace.argtypes = [C.c_int64, C.c_int64, C.POINTER(C.c_uint64)]
+        L.cb200_layer_norm_backward.argtypes = [C.POINTER(LayerNorm), C.c_void_p]
+        L.cb200_qcsr_adapters.argtypes = [C.POINTER(Adapters), C.c_void_p]
         L.cb200_test_arm_wait_timeout.restype = None
         L.cb200_test_arm_wait_timeout.argtypes = [C.c_uint32]
         L.cb200_test_disarm_wait_timeout.restype = None

@@ -1,0 +1,234 @@
+// What the forward and the backward pass of the layer norm share: the checks of a call, how rows are shared out, activations,
+// and sums over a row that lies in one warp's lanes, in one block's threads or in a cluster's.
+#pragma once
+
+#include "counter_random.cuh"
+#include "row_quads.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace cb200 {
+
+// Widths.  Up to kNarrowColumns a row belongs to a group of lanes of one warp; wider ones to a block, or to a cluster of up to
+// eight blocks, each with a slice of the columns.
+constexpr int kNarrowColumns = 512;
+constexpr std::int64_t kMostColumns = 65536;
+constexpr int kNarrowItems = 4;    // quads of a row that a lane holds
+constexpr int kNarrowThreads = 256;
+constexpr int kWideThreads = 576;  // most threads of a block of a wide row
+constexpr int kMostWarps = kWideThreads / 32;
+constexpr int kMostCluster = 8;
+
+struct layer_norm_params {
+    row_matrix x, y, dy, dx;
+    const float *gamma, *beta;
+    float *stats;          // [rows][2]: mean, 1 / standard deviation
+    float *partials;       // backward: [parts][2][columns]
+    std::int64_t rows;
+    int columns;
+    int per_access;        // columns that a load or store of every one of the matrices can take
+    int lanes;             // narrow: lanes of a row, a power of two
+    int slice_quads;       // wide: quads of a block's slice
+    int cluster;           // wide: blocks of a row
+    int epilogue;
+    float epsilon;
+    dropout_args drop;
+};
+
+// How a wide row is cut: quads per thread, blocks of the cluster, threads of a block.
+struct wide_shape {
+    int quads_per_thread, cluster, threads, slice_quads;
+};
+// As few blocks to a row as hold it with two quads to a thread (the sums of a row that one block holds need no cluster barrier;
+// four quads, which halve the resident threads, only where eight blocks do not suffice).
+inline wide_shape wide_shape_of(std::int64_t columns) {
+    wide_shape s{};
+    const int quads = static_cast<int>((columns + 3) / 4);
+    s.quads_per_thread = quads <= 2 * kWideThreads * kMostCluster ? 2 : 4;
+    s.cluster = 1;
+    while (s.cluster < kMostCluster && quads > s.quads_per_thread * kWideThreads * s.cluster) s.cluster *= 2;
+    s.slice_quads = (quads + s.cluster - 1) / s.cluster;
+    s.threads = ((s.slice_quads + s.quads_per_thread - 1) / s.quads_per_thread + 31) / 32 * 32;
+    return s;
+}
+
+// Launches a kernel of a wide row as clusters.
+template<typename K>
+cudaError_t launch_wide(K kernel, const layer_norm_params &p, const wide_shape &shape, unsigned clusters, cudaStream_t stream) {
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(shape.cluster);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(clusters * static_cast<unsigned>(shape.cluster));
+    config.blockDim = dim3(static_cast<unsigned>(shape.threads));
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = shape.cluster > 1 ? 1u : 0u;
+    return cudaLaunchKernelEx(&config, kernel, p);
+}
+
+// Clusters of this shape that the device holds at once, at least one.  Asked for once for each shape (the answer is a
+// property of the kernel and the device).
+template<auto kernel>
+unsigned resident_clusters(const wide_shape &shape, int device) {
+    constexpr int kDevices = 64;
+    static std::atomic<unsigned> known[kDevices][kMostCluster + 1][kMostWarps + 1];
+    const bool kept = device >= 0 && device < kDevices;
+    if (kept) {
+        const unsigned n = known[device][shape.cluster][shape.threads / 32].load(std::memory_order_relaxed);
+        if (n != 0u) return n;
+    }
+    int found = 0;
+    if (shape.cluster > 1) {
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = static_cast<unsigned>(shape.cluster);
+        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(static_cast<unsigned>(shape.cluster));
+        config.blockDim = dim3(static_cast<unsigned>(shape.threads));
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess) found = 0;
+    } else {
+        int per_sm = 0, sms = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, shape.threads, 0) == cudaSuccess &&
+            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess)
+            found = per_sm * sms;
+    }
+    if (found < 1) {
+        cudaGetLastError();
+        return 1u;
+    }
+    if (kept) known[device][shape.cluster][shape.threads / 32].store(static_cast<unsigned>(found), std::memory_order_relaxed);
+    return static_cast<unsigned>(found);
+}
+
+// The lanes of a narrow row: as few as hold it with four quads each, so that its sums need few shuffles and a lane has four
+// loads in flight.
+inline int narrow_lanes(std::int64_t columns) {
+    const std::int64_t quads = (columns + 3) / 4;
+    int lanes = 1;
+    while (lanes < 32 && lanes * kNarrowItems < quads) lanes *= 2;
+    return lanes;
+}
+
+inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward, layer_norm_params *p) {
+    if (d == nullptr || d->version != CB200_ABI_VERSION || d->size < sizeof(cb200_layer_norm))
+        return fail(CB200_STATUS_INVALID_ARGUMENT, "bad cb200_layer_norm header");
+    if (d->rows < 0 || d->columns < 1 || d->columns > kMostColumns || d->rows > (1ll << 32))
+        return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes up to 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns,
+                    (long long)d->rows, (long long)d->columns);
+    if (d->epilogue != CB200_EPILOGUE_NONE && d->epilogue != CB200_EPILOGUE_RELU && d->epilogue != CB200_EPILOGUE_GELU_ERF &&
+        d->epilogue != CB200_EPILOGUE_GELU_TANH)
+        return fail(CB200_STATUS_UNSUPPORTED, "the layer norm's epilogue is none, relu, gelu_erf or gelu_tanh (its bias is beta), got kind %d", d->epilogue);
+    cb200_status st = row_matrix_of(d->x, d->x_ld, d->x_dtype, d->rows, d->columns, "x", &p->x);
+    if (st == CB200_STATUS_SUCCESS) st = dropout_of(&d->dropout, d->rows, &p->drop);
+    if (st != CB200_STATUS_SUCCESS) return st;
+    const float *vectors[] = {d->gamma, d->beta, d->dgamma, d->dbeta};
+    for (const float *v : vectors)
+        if (reinterpret_cast<std::uintptr_t>(v) % 4u != 0u) return fail(CB200_STATUS_INVALID_ARGUMENT, "a vector of parameters is not aligned to its elements");
+    if (reinterpret_cast<std::uintptr_t>(d->stats) % 8u != 0u) return fail(CB200_STATUS_INVALID_ARGUMENT, "stats is not aligned to 8 bytes");
+    p->gamma = d->gamma;
+    p->beta = d->beta;
+    p->stats = d->stats;
+    p->rows = d->rows;
+    p->columns = static_cast<int>(d->columns);
+    p->epilogue = d->epilogue;
+    p->epsilon = d->epsilon;
+    p->lanes = narrow_lanes(d->columns);
+    p->per_access = columns_per_access(p->x, 4);
+    if (!backward && !(d->epsilon >= 0.0f && d->epsilon < 3.4e38f)) return fail(CB200_STATUS_INVALID_ARGUMENT, "epsilon %g is no number from 0 on", d->epsilon);
+    return CB200_STATUS_SUCCESS;
+}
+
+#if defined(__CUDACC__)
+// A quad of a parameter vector; `otherwise` where there is no vector or no column.
+__device__ __forceinline__ void load_parameters(const float *v, int col, int n, float otherwise, float (&out)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = v != nullptr && col + k < n ? __ldg(v + col + k) : otherwise;
+}
+
+// Logistic function: 1 / (1 + e^-t), within a few units of the last place of 1 (the exponential's argument keeps 2^-24 of
+// itself).
+__device__ __forceinline__ float logistic(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
+
+// act(z).  The tanh form of GELU, z / 2 (1 + tanh(c (z + 0.044715 z^3))), is z times the logistic function of twice that argument.
+__device__ __forceinline__ float activation(float z, int kind) {
+    if (kind == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
+    if (kind == CB200_EPILOGUE_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if (kind == CB200_EPILOGUE_GELU_TANH) {
+        const float t = 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f);
+        return z * logistic(t);
+    }
+    return z;
+}
+
+// dy act'(z); relu's slope is 0 at 0, and lets nothing of dy through there
+__device__ __forceinline__ float through_activation(float dy, float z, int kind) {
+    if (kind == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
+    if (kind == CB200_EPILOGUE_GELU_ERF)
+        return dy * fmaf(z, 0.39894228040143268f * __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    const float zz = z * z, gate = logistic(1.5957691216057308f * z * fmaf(0.044715f, zz, 1.0f));
+    const float steep = gate * (1.0f - gate); // 0 far from 0, where the polynomial may be infinite
+    return dy * (steep > 0.0f ? fmaf(z * steep, 1.5957691216057308f * fmaf(0.134145f, zz, 1.0f), gate) : gate);
+}
+
+// Sum over groups of `lanes` neighbouring lanes, in each of them.
+__device__ __forceinline__ float lane_sum(float v, int lanes) {
+    for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Sums of N values over a block, or over a cluster of blocks: each warp leaves its own at every block of the cluster, and after
+// one barrier every warp adds up all of them, in the same order.  The slots are used in turn: what is written for a sum was
+// read for the last but one, and every thread has passed a barrier since.
+template<int N, bool CLUSTER>
+struct wide_sums {
+    float slot[2][kMostCluster * kMostWarps][N];
+
+    __device__ __forceinline__ void add_up(float (&v)[N], int turn, int rank, int cluster) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+        }
+        float *mine = slot[turn][rank * warps + warp];
+        if constexpr (CLUSTER) {
+            if (lane < cluster) {
+                std::uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<std::uint32_t>(__cvta_generic_to_shared(mine))), "r"(lane));
+#pragma unroll
+                for (int k = 0; k < N; ++k) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + 4u * k), "f"(v[k]) : "memory");
+            }
+            cluster_barrier();
+        } else {
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) mine[k] = v[k];
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = 0.0f;
+        for (int i = lane; i < cluster * warps; i += 32) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] += slot[turn][i][k];
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+        }
+    }
+};
+#endif
+
+} // namespace cb200

@@ -456,6 +456,207 @@ def bell_forward(x: QuantizedBell, w: torch.Tensor, out: torch.Tensor | None = N
     return out
 
 
+# ---- behind and beside the projection: dropout, layer norm, adapters ---------------------------
+
+_TORCH_ROWS = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16}
+# The calls' structures as bytes, fields in the order of capi.DropoutMatrix, LayerNorm and Adapters (as _LAUNCH above).  A
+# cb200_dropout is d Q Q P q and starts on 8 bytes.
+_DROPOUT_MATRIX = struct.Struct("@INqqPqPqiidQQPqi4x")
+_LAYER_NORM = struct.Struct("@INqqPqPPiifidQQPqPPqPqPqiii4xPPPQ")
+_ADAPTERS = struct.Struct("@INPPqqqPPPiiPqffPqqi4x")
+assert _DROPOUT_MATRIX.size == C.sizeof(capi.DropoutMatrix)
+assert _LAYER_NORM.size == C.sizeof(capi.LayerNorm)
+assert _ADAPTERS.size == C.sizeof(capi.Adapters)
+_packed_entries: dict = {}
+
+
+def _call_packed(name: str, structure: bytes, device) -> None:
+    """An entry point that takes one structure, as bytes, and the device's current stream."""
+    entry = _packed_entries.get(name)
+    if entry is None:
+        entry = _packed_entries[name] = C.CFUNCTYPE(C.c_int32, C.c_char_p, C.c_void_p)((name, capi.lib()))
+    status = entry(structure, _stream_handle(device))
+    if status:
+        capi.check(status)
+
+
+def _index(device) -> int:
+    return torch.cuda.current_device() if device.index is None else device.index
+
+
+def _rows_of(t: torch.Tensor, name: str, shape=None) -> int:
+    """The type code of a matrix of rows that a row operator takes, which is checked."""
+    code = _TORCH_ROWS.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be a matrix whose rows are contiguous")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    return code
+
+
+def _vector(t: torch.Tensor | None, name: str, length: int, dtype=torch.float32) -> int:
+    """Address of an optional vector, which is checked; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != length or (t.stride(0) != 1 and length > 1):
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {length}")
+    return t.data_ptr()
+
+
+def _together(device, *tensors) -> None:
+    """The operands of a call live on one CUDA device."""
+    if device.type != "cuda":
+        raise ValueError("the operands must be on a CUDA device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands on {t.device} and {device}")
+
+
+def _generator(probability: float, seed: int, sequence: int, first_row: int, device_sequence):
+    """The fields of a cb200_dropout."""
+    if not 0 <= seed < 1 << 64 or not 0 <= sequence < 1 << 64:
+        raise ValueError("seed and sequence are whole numbers below 2^64")
+    if device_sequence is not None and (device_sequence.dtype not in (torch.int64, torch.uint64) or device_sequence.numel() != 1):
+        raise ValueError("device_sequence must be one 64-bit whole number")
+    return probability, seed, sequence, 0 if device_sequence is None else device_sequence.data_ptr(), first_row
+
+
+def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *, first_row: int = 0,
+            device_sequence: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x / (1 - probability) where the counter-based generator keeps the value, else 0 (cb200_dropout_rows).
+
+    The mask follows from probability, seed, sequence (a number for each use), row and column alone: the gradient is the same
+    call on the gradient, and a shard passes the number of its first row.  device_sequence: one int64 on the device that is
+    added to sequence when the kernel runs.  out may be x."""
+    code = _rows_of(x, "x")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out_code = _rows_of(out, "out", x.shape)
+    generator = _generator(probability, seed, sequence, first_row, device_sequence)
+    device = x.device
+    _together(device, out, device_sequence)
+    _call_packed("cb200_dropout_rows", _DROPOUT_MATRIX.pack(
+        capi.ABI_VERSION, _DROPOUT_MATRIX.size, x.shape[0], x.shape[1], x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), code,
+        out_code, *generator, _index(device)), device)
+    return out
+
+
+def _norm_epilogue(epilogue) -> int:
+    return capi.EPILOGUE[epilogue] if isinstance(epilogue, str) else int(epilogue)
+
+
+def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5, *,
+               epilogue: str | int = 0, dropout: float = 0.0, seed: int = 0, sequence: int = 0, first_row: int = 0,
+               device_sequence: torch.Tensor | None = None, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+               stats: torch.Tensor | None = None) -> torch.Tensor:
+    """dropout(act(gamma * (x - mean) / sqrt(var + eps) + beta)), row by row (cb200_layer_norm_forward).
+
+    epilogue: "none", "relu", "gelu_erf" or "gelu_tanh".  The result has x's type, out_dtype or that of out (which may be x).
+    stats, a float32 [rows, 2] tensor, receives each row's {mean, 1 / sqrt(var + eps)}, which layer_norm_backward reads.
+    dropout is a probability; seed, sequence, first_row and device_sequence are those of ops.dropout."""
+    code = _rows_of(x, "x")
+    rows, columns = x.shape
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out has another type than out_dtype")
+    out_code = _rows_of(out, "out", x.shape)
+    gamma_ptr, beta_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns)
+    stats_ptr = 0 if stats is None else _stats_of(stats, rows)
+    generator = _generator(dropout, seed, sequence, first_row, device_sequence)
+    device = x.device
+    _together(device, gamma, beta, out, stats, device_sequence)
+    _call_packed("cb200_layer_norm_forward", _LAYER_NORM.pack(
+        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), x.stride(0), gamma_ptr, beta_ptr, code, _norm_epilogue(epilogue), eps,
+        _index(device), *generator, stats_ptr, out.data_ptr(), out.stride(0), 0, 0, 0, 0, out_code, 0, 0, 0, 0, 0, 0), device)
+    return out
+
+
+def _stats_of(stats: torch.Tensor, rows: int) -> int:
+    if stats.dtype != torch.float32 or stats.shape != (rows, 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be a contiguous float32 tensor of shape ({rows}, 2)")
+    return stats.data_ptr()
+
+
+def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, gamma: torch.Tensor | None = None,
+                        beta: torch.Tensor | None = None, *, epilogue: str | int = 0, dropout: float = 0.0, seed: int = 0,
+                        sequence: int = 0, first_row: int = 0, device_sequence: torch.Tensor | None = None,
+                        dx: torch.Tensor | None = None, dx_dtype: torch.dtype | None = None, dgamma: torch.Tensor | None = None,
+                        dbeta: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """(dx, dgamma, dbeta) of layer_norm with the same arguments, from the gradient dy of its result (cb200_layer_norm_backward).
+
+    dx has x's type, dx_dtype or that of dx (which may be x or dy); spmm_transpose takes it as fp32.  dgamma and dbeta are
+    float32, None where gamma or beta is None.  workspace: a tensor of layer_norm_backward_workspace bytes, else taken from
+    torch's allocator."""
+    code, dy_code = _rows_of(x, "x"), _rows_of(dy, "dy", x.shape)
+    rows, columns = x.shape
+    if dx is None:
+        dx = torch.empty(x.shape, dtype=x.dtype if dx_dtype is None else dx_dtype, device=x.device)
+    elif dx_dtype is not None and dx.dtype != dx_dtype:
+        raise ValueError("dx has another type than dx_dtype")
+    dx_code = _rows_of(dx, "dx", x.shape)
+    gamma_ptr, beta_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns)
+    if dgamma is None and gamma is not None:
+        dgamma = torch.empty(columns, dtype=torch.float32, device=x.device)
+    if dbeta is None and beta is not None:
+        dbeta = torch.empty(columns, dtype=torch.float32, device=x.device)
+    stats_ptr = _stats_of(stats, rows)
+    dgamma_ptr, dbeta_ptr = _vector(dgamma, "dgamma", columns), _vector(dbeta, "dbeta", columns)
+    if workspace is None and (dgamma_ptr or dbeta_ptr):
+        workspace = torch.empty(layer_norm_backward_workspace(rows, columns), dtype=torch.uint8, device=x.device)
+    generator = _generator(dropout, seed, sequence, first_row, device_sequence)
+    device = x.device
+    _together(device, dy, stats, gamma, beta, dx, dgamma, dbeta, workspace, device_sequence)
+    _call_packed("cb200_layer_norm_backward", _LAYER_NORM.pack(
+        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), x.stride(0), gamma_ptr, beta_ptr, code, _norm_epilogue(epilogue), 0.0,
+        _index(device), *generator, stats_ptr, 0, 0, dy.data_ptr(), dy.stride(0), dx.data_ptr(), dx.stride(0), 0, dy_code, dx_code,
+        dgamma_ptr, dbeta_ptr, 0 if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size()), device)
+    return dx, dgamma, dbeta
+
+
+def layer_norm_backward_workspace(rows: int, columns: int) -> int:
+    """Bytes that layer_norm_backward needs for the sums of dgamma and dbeta."""
+    need = C.c_uint64()
+    capi.check(capi.lib().cb200_layer_norm_backward_workspace(rows, columns, C.byref(need)))
+    return need.value
+
+
+def adapter_forward(x: QuantizedCsr, adapter: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None = None, *,
+                    out: torch.Tensor | None = None, alpha=1.0, beta=0.0, row_begin=0, row_end=capi.ALL_ROWS, epilogue: str | int = 0,
+                    bias: torch.Tensor | None = None) -> torch.Tensor:
+    """out[r] = act(alpha * scale[a] * (deq(X)[r] down[a]) up[a] + beta * out[r] + bias) with a = adapter[r], the adapter that row
+    r's request brings; without the product where a is -1 (cb200_qcsr_adapters).
+
+    adapter: int32 [rows]; down [adapters, genes, rank] and up [adapters, rank, n] float32 or bfloat16, contiguous; scale float32
+    [adapters].  With beta=1 and the out of spmm_forward the adapters come on top of the shared projection."""
+    if down.dim() != 3 or up.dim() != 3 or down.dtype not in _TORCH_DENSE or up.dtype != down.dtype:
+        raise ValueError("down and up must be float32 or bfloat16 tensors of three dimensions and one type")
+    adapters, _, rank = down.shape
+    n = up.shape[2]
+    if down.shape[1] != x.cols or up.shape[0] != adapters or up.shape[1] != rank:
+        raise ValueError(f"down must be [adapters, {x.cols}, rank] and up [adapters, rank, n]")
+    if not down.is_contiguous() or not up.is_contiguous():
+        raise ValueError("down and up must be contiguous")
+    adapter_ptr = _vector(adapter, "adapter", x.rows, torch.int32)
+    scale_ptr, bias_ptr = _vector(scale, "scale", adapters), _vector(bias, "bias", n)
+    device = x.device
+    if out is None:
+        if beta != 0.0:
+            raise ValueError("beta needs an out to add to")
+        out = torch.empty(x.rows, n, dtype=torch.float32, device=device)
+    if out.dtype != torch.float32 or out.shape != (x.rows, n) or (out.stride(1) != 1 and n > 1):
+        raise ValueError(f"out must be a float32 matrix of shape ({x.rows}, {n}) whose rows are contiguous")
+    _together(device, adapter, down, up, scale, out, bias)
+    _call_packed("cb200_qcsr_adapters", _ADAPTERS.pack(
+        capi.ABI_VERSION, _ADAPTERS.size, x._bound()[2], adapter_ptr, adapters, rank, n, down.data_ptr(), up.data_ptr(), scale_ptr,
+        _TORCH_DENSE[down.dtype], _norm_epilogue(epilogue), out.data_ptr(), out.stride(0), alpha, beta, bias_ptr, row_begin, row_end,
+        _index(device)), device)
+    return out
+
+
 # ---- CSR -> physical Blocked-ELL lowering on the device ---------------------------------------
 
 class BellLowering:

@@ -675,6 +675,112 @@ cb200_status cb200_qcsr_gene_major(const cb200_qcsr *x, int64_t *col_ptr, int32_
                                    void *workspace, uint64_t workspace_bytes, int32_t device, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * What stands behind and beside the projection in a model (no counterpart in the Cellerator reference, whose
+ * operation core ends with the projection's epilogue): dropout, layer norm with its gradients, and the low-rank
+ * adapters of many requests.  Dense operands are row-major with leading dimensions in elements, fp32, bf16 or fp16
+ * (CB200_DTYPE_*), any width and any alignment of at least one element.  Sums and statistics are fp32; a result of
+ * fewer bits is rounded once, to nearest.  The calls check their arguments, enqueue on `stream`, allocate nothing and
+ * do not synchronise; they can be captured into graphs.  The same arguments give the same bits on every call. */
+
+/* Dropout from a counter-based generator, with a mask that is never stored.  Value (row, column) of a call is dropped
+ * when its random word is below round(probability * 2^32), else multiplied by 1 / (1 - probability); a dropped value is
+ * zero whatever it was.  The word is word column % 4 of Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC'11) with counter
+ * {column / 4, first_row + row, sequence (low, high 32 bits)} and key = seed (low, high): it does not depend on the
+ * layout, and a shard that names its first row drops what the whole matrix would.  Calls that must not share a mask take
+ * different sequences. */
+typedef struct cb200_dropout {
+    double probability; /* in [0, 1); 0: every value is kept */
+    uint64_t seed;
+    uint64_t sequence;
+    const uint64_t *device_sequence; /* optional, on the device: read by the kernels and added to `sequence`, for a captured
+                                      * call whose mask is to change from replay to replay */
+    int64_t first_row;               /* number of row 0; first_row + rows <= 2^32 */
+} cb200_dropout;
+
+/* y = dropout(x) over rows x columns; y may be x (same leading dimension, elements of the same size), else they share no
+ * byte.  The gradient is the same call on the gradient of y. */
+typedef struct cb200_dropout_matrix {
+    uint32_t version;
+    size_t size;
+    int64_t rows, columns;
+    const void *x;
+    int64_t x_ld;
+    void *y;
+    int64_t y_ld;
+    int32_t x_dtype, y_dtype;
+    cb200_dropout dropout;
+    int32_t device;
+} cb200_dropout_matrix;
+
+cb200_status cb200_dropout_rows(const cb200_dropout_matrix *matrix, void *stream);
+
+/* Layer norm over the columns of each row, with the activation and dropout that follow it in the same pass:
+ *     u = (x - mean) / sqrt(var + epsilon),  z = gamma u + beta,  y = dropout(act(z)),
+ * var the mean of the squared differences.  epilogue: CB200_EPILOGUE_NONE, _RELU, _GELU_ERF or _GELU_TANH (beta is the
+ * bias).  1 to 65,536 columns, up to 2^32 rows; more are refused.
+ * Forward writes y (which may be x, as for dropout) and, when asked, stats.
+ * Backward reads x, dy and the stats of the forward call with the same parameters, epilogue and dropout, and writes
+ * those of dx (which may be x or dy), dgamma and dbeta that are not NULL; relu's slope is 0 at 0.  It needs
+ * cb200_layer_norm_backward_workspace bytes (4-byte aligned) when dgamma or dbeta is wanted: two sums per column of
+ * every part that the rows are cut into, which a second launch adds up in a fixed order. */
+typedef struct cb200_layer_norm {
+    uint32_t version;
+    size_t size;
+    int64_t rows, columns;
+    const void *x;
+    int64_t x_ld;
+    const float *gamma, *beta; /* columns each; NULL: 1 and 0 */
+    int32_t x_dtype;
+    int32_t epilogue;
+    float epsilon;     /* forward */
+    int32_t device;
+    cb200_dropout dropout;
+    float *stats;      /* rows x {mean, 1 / sqrt(var + epsilon)}, 8-byte aligned; forward: or NULL */
+    void *y;           /* forward */
+    int64_t y_ld;
+    const void *dy;    /* backward */
+    int64_t dy_ld;
+    void *dx;          /* backward; or NULL */
+    int64_t dx_ld;
+    int32_t y_dtype, dy_dtype, dx_dtype;
+    float *dgamma, *dbeta; /* backward; or NULL */
+    void *workspace;
+    uint64_t workspace_bytes;
+} cb200_layer_norm;
+
+cb200_status cb200_layer_norm_forward(const cb200_layer_norm *norm, void *stream);
+cb200_status cb200_layer_norm_backward_workspace(int64_t rows, int64_t columns, uint64_t *bytes);
+cb200_status cb200_layer_norm_backward(const cb200_layer_norm *norm, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection: row r of a quantized CSR batch belongs to a request that
+ * brings adapter a = adapter[r], two factors down[a] (genes x rank) and up[a] (rank x n):
+ *     out[r] = act(alpha * scale[a] * (deq(X)[r] down[a]) up[a] + beta * out[r] + bias),
+ * and without the product where adapter[r] is -1 (or any value outside 0 .. adapters - 1).  beta == 0 never reads out.
+ * After a cb200_spmm_run into the same out, beta = 1 adds the adapters to the shared projection, and the epilogue is then
+ * this call's; products and sums are fp32.  A gene outside the matrix is left out.  A row's bits follow from its
+ * entries, its adapter and the types, not from the rows beside it. */
+typedef struct cb200_adapters {
+    uint32_t version;
+    size_t size;
+    const cb200_qcsr *csr;  /* 8- or 4-bit codes */
+    const int32_t *adapter; /* device, one per row of the matrix */
+    int64_t adapters, rank, n; /* rank 1 .. 256 */
+    const void *down;       /* device, adapters x genes x rank, contiguous */
+    const void *up;         /* device, adapters x rank x n, contiguous */
+    const float *scale;     /* device, one per adapter; NULL: 1 */
+    int32_t weight_dtype;   /* of down and up: CB200_DTYPE_F32 or CB200_DTYPE_BF16 */
+    int32_t epilogue;       /* cb200_epilogue; the bias kinds read bias */
+    float *out;             /* device, fp32, rows indexed by absolute row */
+    int64_t out_ld;
+    float alpha, beta;
+    const float *bias;      /* device, n */
+    int64_t row_begin, row_end; /* as in cb200_launch */
+    int32_t device;
+} cb200_adapters;
+
+cb200_status cb200_qcsr_adapters(const cb200_adapters *adapters, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Routing of the reference's public projection calls: cellerator_sparse_projection_forward /
  * _backward (include/Cellerator/abi.h:111-124, src/abi/abi.cu:278-396) for the quantized layouts,
  * which the reference declares (CELLERATOR_LAYOUT_QUANTIZED_BLOCKED_ELL, abi.h:31-36) and rejects
