@@ -14,7 +14,7 @@ namespace cb200 {
 struct dropout_args {
     std::uint32_t threshold = 0u;
     float scale = 1.0f;
-    std::uint32_t key0 = 0u, key1 = 0u;
+    std::uint32_t key[10][2] = {}; // of the rounds: the same for every value, so they are operands out of the launch's constants
     std::uint64_t sequence = 0u;
     const std::uint64_t *device_sequence = nullptr;
     std::uint32_t first_row = 0u;
@@ -34,8 +34,10 @@ inline cb200_status dropout_of(const cb200_dropout *d, std::int64_t rows, dropou
     const double threshold = std::floor(d->probability * 4294967296.0 + 0.5);
     out->threshold = threshold >= 4294967295.0 ? 0xffffffffu : static_cast<std::uint32_t>(threshold);
     out->scale = static_cast<float>(1.0 / (1.0 - d->probability));
-    out->key0 = static_cast<std::uint32_t>(d->seed);
-    out->key1 = static_cast<std::uint32_t>(d->seed >> 32);
+    for (std::uint32_t round = 0; round < 10; ++round) {
+        out->key[round][0] = static_cast<std::uint32_t>(d->seed) + round * 0x9E3779B9u;
+        out->key[round][1] = static_cast<std::uint32_t>(d->seed >> 32) + round * 0xBB67AE85u;
+    }
     out->sequence = d->sequence;
     out->device_sequence = d->device_sequence;
     out->first_row = static_cast<std::uint32_t>(d->first_row);
@@ -48,21 +50,17 @@ __device__ __forceinline__ std::uint64_t sequence_of(const dropout_args &d) {
     return d.sequence + (d.device_sequence != nullptr ? *d.device_sequence : 0u);
 }
 
-// The words of columns 4 * quad ... 4 * quad + 3 of a row.  A round is two 32 x 32 -> 64-bit products and two three-way xors;
-// the round keys are the same for every value of a launch.
+// The words of columns 4 * quad ... 4 * quad + 3 of a row.  A round is two 32 x 32 -> 64-bit products and two three-way xors.
 __device__ __forceinline__ void random_words(const dropout_args &d, std::uint64_t sequence, std::uint32_t row, std::uint32_t quad,
                                              std::uint32_t (&word)[4]) {
     std::uint32_t a = quad, b = row, c = static_cast<std::uint32_t>(sequence), e = static_cast<std::uint32_t>(sequence >> 32);
-    std::uint32_t k0 = d.key0, k1 = d.key1;
 #pragma unroll
     for (int round = 0; round < 10; ++round) {
         const std::uint64_t p = static_cast<std::uint64_t>(a) * 0xD2511F53u, q = static_cast<std::uint64_t>(c) * 0xCD9E8D57u;
-        a = static_cast<std::uint32_t>(q >> 32) ^ b ^ k0;
+        a = static_cast<std::uint32_t>(q >> 32) ^ b ^ d.key[round][0];
         b = static_cast<std::uint32_t>(q);
-        c = static_cast<std::uint32_t>(p >> 32) ^ e ^ k1;
+        c = static_cast<std::uint32_t>(p >> 32) ^ e ^ d.key[round][1];
         e = static_cast<std::uint32_t>(p);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     word[0] = a; word[1] = b; word[2] = c; word[3] = e;
 }

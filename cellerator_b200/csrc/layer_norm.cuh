@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace cb200 {
 
@@ -14,10 +15,11 @@ namespace cb200 {
 // eight blocks, each with a slice of the columns.
 constexpr int kNarrowColumns = 512;
 constexpr std::int64_t kMostColumns = 65536;
-constexpr int kNarrowItems = 4;    // quads of a row that a lane holds
 constexpr int kNarrowThreads = 256;
-constexpr int kWideThreads = 576;  // most threads of a block of a wide row
-constexpr int kMostWarps = kWideThreads / 32;
+// Most threads of a block of a wide row, by the quads of a thread.  Three quads and twelve warps: three warps to a scheduler leave
+// each thread 168 registers, and eight such blocks hold 36,864 columns.
+constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 3 ? 384 : 512; }
+constexpr int kMostWarps = 16;
 constexpr int kMostCluster = 8;
 
 struct layer_norm_params {
@@ -40,14 +42,14 @@ struct layer_norm_params {
 struct wide_shape {
     int quads_per_thread, cluster, threads, slice_quads;
 };
-// As few blocks to a row as hold it with two quads to a thread (the sums of a row that one block holds need no cluster barrier;
-// four quads, which halve the resident threads, only where eight blocks do not suffice).
+// As few blocks to a row as hold it (the sums of a row that one block holds need no cluster barrier), with three quads to a thread
+// where eight blocks suffice.
 inline wide_shape wide_shape_of(std::int64_t columns) {
     wide_shape s{};
     const int quads = static_cast<int>((columns + 3) / 4);
-    s.quads_per_thread = quads <= 2 * kWideThreads * kMostCluster ? 2 : 4;
+    s.quads_per_thread = quads <= 3 * wide_threads(3) * kMostCluster ? 3 : 4;
     s.cluster = 1;
-    while (s.cluster < kMostCluster && quads > s.quads_per_thread * kWideThreads * s.cluster) s.cluster *= 2;
+    while (s.cluster < kMostCluster && quads > s.quads_per_thread * wide_threads(s.quads_per_thread) * s.cluster) s.cluster *= 2;
     s.slice_quads = (quads + s.cluster - 1) / s.cluster;
     s.threads = ((s.slice_quads + s.quads_per_thread - 1) / s.quads_per_thread + 31) / 32 * 32;
     return s;
@@ -106,20 +108,21 @@ unsigned resident_clusters(const wide_shape &shape, int device) {
     return static_cast<unsigned>(found);
 }
 
-// The lanes of a narrow row: as few as hold it with four quads each, so that its sums need few shuffles and a lane has four
-// loads in flight.
+// A narrow row: quads that a lane holds, and lanes of the row, as few as hold it (its sums then take few shuffles).  Two quads
+// up to 256 columns, so that the backward pass, which keeps four numbers a column, has room for 24 warps an SM.
+inline int narrow_items(std::int64_t columns) { return columns <= 256 ? 2 : 4; }
 inline int narrow_lanes(std::int64_t columns) {
     const std::int64_t quads = (columns + 3) / 4;
     int lanes = 1;
-    while (lanes < 32 && lanes * kNarrowItems < quads) lanes *= 2;
+    while (lanes < 32 && lanes * narrow_items(columns) < quads) lanes *= 2;
     return lanes;
 }
 
 inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward, layer_norm_params *p) {
     if (d == nullptr || d->version != CB200_ABI_VERSION || d->size < sizeof(cb200_layer_norm))
         return fail(CB200_STATUS_INVALID_ARGUMENT, "bad cb200_layer_norm header");
-    if (d->rows < 0 || d->columns < 1 || d->columns > kMostColumns || d->rows > (1ll << 32))
-        return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes up to 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns,
+    if (d->rows < 0 || d->columns < 1 || d->columns > kMostColumns || d->rows >= (1ll << 32))
+        return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes fewer than 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns,
                     (long long)d->rows, (long long)d->columns);
     if (d->epilogue != CB200_EPILOGUE_NONE && d->epilogue != CB200_EPILOGUE_RELU && d->epilogue != CB200_EPILOGUE_GELU_ERF &&
         d->epilogue != CB200_EPILOGUE_GELU_TANH)
@@ -144,6 +147,17 @@ inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward,
     return CB200_STATUS_SUCCESS;
 }
 
+// Calls f with the epilogue as a constant.
+template<typename F>
+cb200_status with_epilogue(int kind, F f) {
+    switch (kind) {
+    case CB200_EPILOGUE_RELU: return f(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
+    case CB200_EPILOGUE_GELU_ERF: return f(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
+    case CB200_EPILOGUE_GELU_TANH: return f(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
+    default: return f(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
+    }
+}
+
 #if defined(__CUDACC__)
 // A quad of a parameter vector; `otherwise` where there is no vector or no column.
 __device__ __forceinline__ void load_parameters(const float *v, int col, int n, float otherwise, float (&out)[4]) {
@@ -156,24 +170,26 @@ __device__ __forceinline__ void load_parameters(const float *v, int col, int n, 
 __device__ __forceinline__ float logistic(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
 
 // act(z).  The tanh form of GELU, z / 2 (1 + tanh(c (z + 0.044715 z^3))), is z times the logistic function of twice that argument.
-__device__ __forceinline__ float activation(float z, int kind) {
-    if (kind == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
-    if (kind == CB200_EPILOGUE_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    if (kind == CB200_EPILOGUE_GELU_TANH) {
-        const float t = 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f);
-        return z * logistic(t);
-    }
+template<int KIND>
+__device__ __forceinline__ float activation(float z) {
+    if constexpr (KIND == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
+    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return z * logistic(1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f));
     return z;
 }
 
 // dy act'(z); relu's slope is 0 at 0, and lets nothing of dy through there
-__device__ __forceinline__ float through_activation(float dy, float z, int kind) {
-    if (kind == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
-    if (kind == CB200_EPILOGUE_GELU_ERF)
+template<int KIND>
+__device__ __forceinline__ float through_activation(float dy, float z) {
+    if constexpr (KIND == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
+    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF)
         return dy * fmaf(z, 0.39894228040143268f * __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
-    const float zz = z * z, gate = logistic(1.5957691216057308f * z * fmaf(0.044715f, zz, 1.0f));
-    const float steep = gate * (1.0f - gate); // 0 far from 0, where the polynomial may be infinite
-    return dy * (steep > 0.0f ? fmaf(z * steep, 1.5957691216057308f * fmaf(0.134145f, zz, 1.0f), gate) : gate);
+    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) {
+        const float zz = z * z, gate = logistic(1.5957691216057308f * z * fmaf(0.044715f, zz, 1.0f));
+        const float steep = gate * (1.0f - gate); // 0 far from 0, where the polynomial may be infinite
+        return dy * (steep > 0.0f ? fmaf(z * steep, 1.5957691216057308f * fmaf(0.134145f, zz, 1.0f), gate) : gate);
+    }
+    return dy;
 }
 
 // Sum over groups of `lanes` neighbouring lanes, in each of them.
@@ -182,25 +198,31 @@ __device__ __forceinline__ float lane_sum(float v, int lanes) {
     return v;
 }
 
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The columns of a thread of a wide row: quad i of the thread starts at column col[i] (the number of columns where it has none).
+template<int QT>
+__device__ __forceinline__ void wide_columns(const layer_norm_params &p, int rank, int (&col)[QT]) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const int quad = i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
+        col[i] = quad < p.slice_quads ? min((rank * p.slice_quads + quad) * 4, p.columns) : p.columns;
+    }
 }
 
-// Sums of N values over a block, or over a cluster of blocks: each warp leaves its own at every block of the cluster, and after
-// one barrier every warp adds up all of them, in the same order.  The slots are used in turn: what is written for a sum was
-// read for the last but one, and every thread has passed a barrier since.
+// What the warps of a block, or of a cluster of blocks, tell each other of a step of rows: N numbers a warp.  A warp leaves its
+// numbers with every block, and behind a barrier every warp reads all of them, in the same order.  A cluster works on one step's
+// numbers while the next one's are on their way, so that three sets are in use: what is written for a step was read three steps
+// before, and every thread has passed a barrier since.
 template<int N, bool CLUSTER>
-struct wide_sums {
-    float slot[2][kMostCluster * kMostWarps][N];
+struct wide_notes {
+    static constexpr int kSets = CLUSTER ? 3 : 2;
+    float note[kSets][(CLUSTER ? kMostCluster : 1) * kMostWarps][N];
 
-    __device__ __forceinline__ void add_up(float (&v)[N], int turn, int rank, int cluster) {
+    __device__ __forceinline__ void leave(const float (&v)[N], int set, int rank, int cluster) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
-        }
-        float *mine = slot[turn][rank * warps + warp];
+        float *mine = note[set][rank * warps + warp];
         if constexpr (CLUSTER) {
             if (lane < cluster) {
                 std::uint32_t there;
@@ -208,27 +230,22 @@ struct wide_sums {
 #pragma unroll
                 for (int k = 0; k < N; ++k) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + 4u * k), "f"(v[k]) : "memory");
             }
-            cluster_barrier();
-        } else {
-            if (lane == 0) {
+        } else if (lane == 0) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) mine[k] = v[k];
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = 0.0f;
-        for (int i = lane; i < cluster * warps; i += 32) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) v[k] += slot[turn][i][k];
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+            for (int k = 0; k < N; ++k) mine[k] = v[k];
         }
     }
 };
+__device__ __forceinline__ int next_set(int set, int sets) { return set + 1 == sets ? 0 : set + 1; }
+
+template<int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N]) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+    }
+}
 #endif
 
 } // namespace cb200

@@ -10,20 +10,21 @@ namespace cb200 {
 namespace {
 
 // Most blocks (narrow) or clusters (wide) of a launch: each leaves 2 x columns sums.
-constexpr int kNarrowParts = 148 * 2;
+constexpr int kNarrowBlocks = 3; // narrow: resident on an SM, with two quads a lane; one less with four
+constexpr int kNarrowParts = 148 * kNarrowBlocks;
 constexpr int kWideParts = 148 * 4;
 
 // dz and u of a quad in place of dy and x; h u added to sums[1], h to sums[0]
+template<int KIND>
 struct quad_terms {
     float mean, rstd;
-    int epilogue;
 
     __device__ __forceinline__ void apply(float (&x)[4], float (&dy)[4], const float (&gamma)[4], const float (&beta)[4], float (&dgamma)[4],
                                           float (&dbeta)[4], float (&sums)[2]) const {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             x[k] = (x[k] - mean) * rstd;
-            if (epilogue != CB200_EPILOGUE_NONE) dy[k] = through_activation(dy[k], fmaf(x[k], gamma[k], beta[k]), epilogue);
+            dy[k] = through_activation<KIND>(dy[k], fmaf(x[k], gamma[k], beta[k]));
             dbeta[k] += dy[k];
             dgamma[k] = fmaf(dy[k], x[k], dgamma[k]);
             dy[k] *= gamma[k];
@@ -33,59 +34,71 @@ struct quad_terms {
     }
 };
 
-// A group of p.lanes lanes per row.  Columns past the last hold zeros in x and dy, so that u there is not zero but dz is.
-template<int SX, int SG>
-__global__ void __launch_bounds__(kNarrowThreads) layer_norm_back_narrow_kernel(const layer_norm_params p) {
-    __shared__ float meet[kNarrowThreads / 32][kNarrowItems * 4 * 32];
+// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  Columns past the last hold
+// zeros in dy, so that they add nothing.
+template<int SX, int SG, int KIND, int ITEMS>
+__global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : kNarrowBlocks - 1) layer_norm_back_narrow_kernel(const layer_norm_params p) {
+    __shared__ float meet[kNarrowThreads / 32][ITEMS * 4 * 32];
+    __shared__ __align__(16) float parameters[2][ITEMS * 4 * 32]; // gamma and beta: registers are short here
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
     const bool half = p.x.dtype == CB200_DTYPE_F16, half_dy = p.dy.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    float gamma[kNarrowItems][4], beta[kNarrowItems][4], dgamma[kNarrowItems][4], dbeta[kNarrowItems][4];
-    int col[kNarrowItems];
+    for (int c = threadIdx.x; c < ITEMS * 4 * 32; c += kNarrowThreads) {
+        parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
+        parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
+    }
+    __syncthreads();
+    float dgamma[ITEMS][4], dbeta[ITEMS][4];
+    int col[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kNarrowItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         col[i] = min((i * p.lanes + in_row) * 4, p.columns);
-        load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
-        load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) dgamma[i][k] = dbeta[i][k] = 0.0f;
     }
     const float inverse = 1.0f / static_cast<float>(p.columns);
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
-    for (std::int64_t base = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + warp) * rows_per_warp; base < p.rows; base += step) {
-        const std::int64_t row = base + group;
-        const bool active = row < p.rows;
-        raw_quad<SX> raw_x[kNarrowItems];
-        raw_quad<SG> raw_dy[kNarrowItems];
-        quad_terms terms{0.0f, 0.0f, p.epilogue};
-        if (active) {
-            const float2 s = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
-            terms.mean = s.x;
-            terms.rstd = s.y;
-        }
+    std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + warp) * rows_per_warp + group;
+    raw_quad<SX> raw_x[ITEMS];
+    raw_quad<SG> raw_dy[ITEMS];
+    float2 stats = make_float2(0.0f, 0.0f);
+    const auto fetch = [&](std::int64_t at) {
+        if (at < p.rows) stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             raw_x[i].clear();
             raw_dy[i].clear();
-            if (active) {
-                raw_x[i].load(p.x.base + row * p.x.pitch, col[i], p.columns, p.per_access);
-                raw_dy[i].load(p.dy.base + row * p.dy.pitch, col[i], p.columns, p.per_access);
+            if (at < p.rows) {
+                raw_x[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
+                raw_dy[i].load(p.dy.base + at * p.dy.pitch, col[i], p.columns, p.per_access);
             }
         }
-        float x[kNarrowItems][4], dy[kNarrowItems][4], sums[2] = {0.0f, 0.0f};
+    };
+    fetch(row);
+    for (; row - group < p.rows; row += step) {
+        const bool active = row < p.rows;
+        const quad_terms<KIND> terms{stats.x, stats.y};
+        float x[ITEMS][4], dy[ITEMS][4], sums[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             raw_x[i].widen(half, x[i]);
             raw_dy[i].widen(half_dy, dy[i]);
+        }
+        fetch(row + step);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
             if (!active || col[i] >= p.columns) continue;
             if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), dy[i]);
-            terms.apply(x[i], dy[i], gamma[i], beta[i], dgamma[i], dbeta[i], sums);
+            float gamma[4], beta[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            *reinterpret_cast<float4 *>(gamma) = *reinterpret_cast<const float4 *>(parameters[0] + col[i]);
+            if constexpr (KIND != CB200_EPILOGUE_NONE) *reinterpret_cast<float4 *>(beta) = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
+            terms.apply(x[i], dy[i], gamma, beta, dgamma[i], dbeta[i], sums);
         }
         sums[0] = lane_sum(sums[0], p.lanes) * inverse;
         sums[1] = lane_sum(sums[1], p.lanes) * inverse;
         if (!active || p.dx.base == nullptr) continue;
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             if (col[i] >= p.columns) continue;
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[i][k] = terms.rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
@@ -98,7 +111,7 @@ __global__ void __launch_bounds__(kNarrowThreads) layer_norm_back_narrow_kernel(
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float v = which == 0 ? dgamma[i][k] : dbeta[i][k];
@@ -118,20 +131,21 @@ __global__ void __launch_bounds__(kNarrowThreads) layer_norm_back_narrow_kernel(
     }
 }
 
-// A block or a cluster of blocks per row, each block with a slice of the columns, whose sums its threads keep from row to row.
-template<int SX, int SG, int QT, bool CLUSTER>
-__global__ void __launch_bounds__(kWideThreads) layer_norm_back_wide_kernel(const layer_norm_params p) {
-    __shared__ wide_sums<2, CLUSTER> around;
+// A block, or a cluster of blocks that take a slice of the columns each, per row; a thread keeps the sums of its columns from row
+// to row.  In a cluster the two sums of a row go round while the row before is written and the one behind is worked on.
+template<int SX, int SG, int KIND, int QT, bool CLUSTER>
+__global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(const layer_norm_params p) {
+    __shared__ wide_notes<2, CLUSTER> notes;
+    const int lane = threadIdx.x & 31, all_warps = p.cluster * (blockDim.x >> 5);
     const int rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
-    const std::int64_t first = CLUSTER ? blockIdx.x / p.cluster : blockIdx.x, step = CLUSTER ? gridDim.x / p.cluster : gridDim.x;
+    const std::int64_t first = CLUSTER ? blockIdx.x / p.cluster : blockIdx.x, stride = CLUSTER ? gridDim.x / p.cluster : gridDim.x;
     const bool half = p.x.dtype == CB200_DTYPE_F16, half_dy = p.dy.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
     float gamma[QT][4], beta[QT][4], dgamma[QT][4], dbeta[QT][4];
     int col[QT];
+    wide_columns<QT>(p, rank, col);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        const int quad = i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
-        col[i] = quad < p.slice_quads ? min((rank * p.slice_quads + quad) * 4, p.columns) : p.columns;
         load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
         load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
 #pragma unroll
@@ -140,46 +154,92 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_back_wide_kernel(cons
     const float inverse = 1.0f / static_cast<float>(p.columns);
     raw_quad<SX> raw_x[QT];
     raw_quad<SG> raw_dy[QT];
-    float2 stats = *reinterpret_cast<const float2 *>(p.stats + 2 * first);
+    float2 stats;
+    const auto fetch = [&](std::int64_t at) {
+        if (at >= p.rows) return;
+        stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        raw_x[i].load(p.x.base + first * p.x.pitch, col[i], p.columns, p.per_access);
-        raw_dy[i].load(p.dy.base + first * p.dy.pitch, col[i], p.columns, p.per_access);
-    }
-    if constexpr (CLUSTER) cluster_barrier(); // every block of the cluster has begun
-    int turn = 0;
-    for (std::int64_t row = first; row < p.rows; row += step, turn ^= 1) {
-        const quad_terms terms{stats.x, stats.y, p.epilogue};
-        float x[QT][4], dy[QT][4], sums[2] = {0.0f, 0.0f};
+        for (int i = 0; i < QT; ++i) {
+            raw_x[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
+            raw_dy[i].load(p.dy.base + at * p.dy.pitch, col[i], p.columns, p.per_access);
+        }
+    };
+    float x[QT][4], dy[QT][4]; // x and dy of a row, then its u and h
+    const auto widened = [&]() {
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             raw_x[i].widen(half, x[i]);
             raw_dy[i].widen(half_dy, dy[i]);
         }
-        if (row + step < p.rows) {
-            stats = *reinterpret_cast<const float2 *>(p.stats + 2 * (row + step));
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                raw_x[i].load(p.x.base + (row + step) * p.x.pitch, col[i], p.columns, p.per_access);
-                raw_dy[i].load(p.dy.base + (row + step) * p.dy.pitch, col[i], p.columns, p.per_access);
-            }
-        }
+    };
+    const auto summed = [&](std::int64_t row, float2 of_row, float (&sums)[2]) {
+        const quad_terms<KIND> terms{of_row.x, of_row.y};
+        sums[0] = sums[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             if (col[i] >= p.columns) continue;
             if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), dy[i]);
             terms.apply(x[i], dy[i], gamma[i], beta[i], dgamma[i], dbeta[i], sums);
         }
-        around.add_up(sums, turn, rank, p.cluster);
-        if (p.dx.base == nullptr) continue;
+        warp_sums<2>(sums);
+    };
+    const auto finish = [&](const float (&u)[QT][4], const float (&h)[QT][4], std::int64_t row, float rstd, int set) {
+        if (p.dx.base == nullptr) return;
+        float sums[2] = {0.0f, 0.0f};
+        for (int w = lane; w < all_warps; w += 32) {
+            sums[0] += notes.note[set][w][0];
+            sums[1] += notes.note[set][w][1];
+        }
+        warp_sums<2>(sums);
         sums[0] *= inverse;
         sums[1] *= inverse;
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             if (col[i] >= p.columns) continue;
+            float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][k] = terms.rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
-            store_quad(p.dx.base + row * p.dx.pitch, col[i], p.columns, p.per_access, p.dx.dtype, x[i]);
+            for (int k = 0; k < 4; ++k) v[k] = rstd * (h[i][k] - sums[0] - u[i][k] * sums[1]);
+            store_quad(p.dx.base + row * p.dx.pitch, col[i], p.columns, p.per_access, p.dx.dtype, v);
+        }
+    };
+    fetch(first);
+    int set = 0;
+    float sums[2];
+    if constexpr (CLUSTER) {
+        float u[QT][4], h[QT][4], rstd = 0.0f; // of the row before
+        cluster_arrive();                      // every block of the cluster has begun
+        std::int64_t row = first;
+        for (; row < p.rows; row += stride) {
+            widened();
+            const float2 of_row = stats;
+            summed(row, of_row, sums);
+            cluster_wait();
+            notes.leave(sums, set, rank, p.cluster);
+            cluster_arrive();
+            fetch(row + stride);
+            if (row != first) finish(u, h, row - stride, rstd, set == 0 ? 2 : set - 1);
+            set = next_set(set, 3);
+            rstd = of_row.y;
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    u[i][k] = x[i][k];
+                    h[i][k] = dy[i][k];
+                }
+            }
+        }
+        cluster_wait();
+        if (row != first) finish(u, h, row - stride, rstd, set == 0 ? 2 : set - 1);
+    } else {
+        for (std::int64_t row = first; row < p.rows; row += stride, set ^= 1) {
+            widened();
+            const float2 of_row = stats;
+            fetch(row + stride);
+            summed(row, of_row, sums);
+            notes.leave(sums, set, rank, p.cluster);
+            __syncthreads();
+            finish(x, dy, row, of_row.y, set);
         }
     }
     let_next_launch_start();
@@ -217,6 +277,12 @@ __global__ void __launch_bounds__(kMeetWarps * 32) layer_norm_meet_kernel(const 
     if (out != nullptr) out[c < columns ? c : c - columns] = v;
 }
 
+// Blocks of a launch over narrow rows.
+std::int64_t narrow_parts(std::int64_t rows, std::int64_t columns) {
+    const std::int64_t per_block = kNarrowThreads / narrow_lanes(columns);
+    return std::min<std::int64_t>((rows + per_block - 1) / per_block, narrow_items(columns) == 2 ? kNarrowParts : kNarrowParts / kNarrowBlocks * (kNarrowBlocks - 1));
+}
+
 struct backward_launch {
     layer_norm_params p;
     float *dgamma, *dbeta;
@@ -238,25 +304,25 @@ struct backward_launch {
         CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(parts), stream));
         return finish(parts);
     }
-    template<int SX, int SG>
+    template<int SX, int SG, int KIND>
     cb200_status run() {
         if (p.columns <= kNarrowColumns) {
-            const std::int64_t per_block = kNarrowThreads / p.lanes, parts = std::min<std::int64_t>((p.rows + per_block - 1) / per_block, kNarrowParts);
-            layer_norm_back_narrow_kernel<SX, SG><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            const std::int64_t parts = narrow_parts(p.rows, p.columns);
+            if (narrow_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            else layer_norm_back_narrow_kernel<SX, SG, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             return finish(parts);
         }
         const wide_shape shape = wide_shape_of(p.columns);
         p.cluster = shape.cluster;
         p.slice_quads = shape.slice_quads;
-        if (shape.cluster == 1) return wide<layer_norm_back_wide_kernel<SX, SG, 2, false>>(shape);
-        if (shape.quads_per_thread == 2) return wide<layer_norm_back_wide_kernel<SX, SG, 2, true>>(shape);
-        return wide<layer_norm_back_wide_kernel<SX, SG, 4, true>>(shape);
+        if (shape.cluster == 1) return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 3, false>>(shape);
+        if (shape.quads_per_thread == 3) return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 3, true>>(shape);
+        return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 4, true>>(shape);
     }
 };
 
 std::uint64_t partial_bytes(std::int64_t rows, std::int64_t columns) {
-    const std::int64_t parts = columns <= kNarrowColumns ? std::min<std::int64_t>((rows + kNarrowThreads / narrow_lanes(columns) - 1) / (kNarrowThreads / narrow_lanes(columns)), kNarrowParts)
-                                                         : std::min<std::int64_t>(rows, kWideParts / wide_shape_of(columns).cluster);
+    const std::int64_t parts = columns <= kNarrowColumns ? narrow_parts(rows, columns) : std::min<std::int64_t>(rows, kWideParts / wide_shape_of(columns).cluster);
     return static_cast<std::uint64_t>(parts) * 2u * static_cast<std::uint64_t>(columns) * sizeof(float);
 }
 
@@ -267,8 +333,8 @@ extern "C" cb200_status cb200_layer_norm_backward_workspace(int64_t rows, int64_
     using namespace cb200;
     clear_error();
     if (bytes == nullptr) return fail(CB200_STATUS_INVALID_ARGUMENT, "workspace needs an output");
-    if (rows < 0 || columns < 1 || columns > kMostColumns || rows > (1ll << 32))
-        return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes up to 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns, (long long)rows, (long long)columns);
+    if (rows < 0 || columns < 1 || columns > kMostColumns || rows >= (1ll << 32))
+        return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes fewer than 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns, (long long)rows, (long long)columns);
     *bytes = partial_bytes(rows, columns);
     return CB200_STATUS_SUCCESS;
 }
@@ -309,6 +375,8 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
     }
     if (!sums && p.dx.base == nullptr) return CB200_STATUS_SUCCESS;
     const bool wide_x = element_bytes(p.x.dtype) == 4, wide_dy = element_bytes(p.dy.dtype) == 4;
-    if (wide_x) return wide_dy ? b.run<4, 4>() : b.run<4, 2>();
-    return wide_dy ? b.run<2, 4>() : b.run<2, 2>();
+    return with_epilogue(p.epilogue, [&](auto kind) {
+        if (wide_x) return wide_dy ? b.run<4, 4, kind()>() : b.run<4, 2, kind()>();
+        return wide_dy ? b.run<2, 4, kind()>() : b.run<2, 2, kind()>();
+    });
 }

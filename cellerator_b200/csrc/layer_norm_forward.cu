@@ -7,138 +7,260 @@
 namespace cb200 {
 namespace {
 
-__device__ __forceinline__ bool held(int col, int k, int n, bool tail) { return tail ? col + k < n : col < n; }
+constexpr int kNarrowBlocks = 4; // resident on an SM
 
-// A group of p.lanes lanes per row.
-template<int SIZE, bool TAIL>
-__global__ void __launch_bounds__(kNarrowThreads) layer_norm_narrow_kernel(const layer_norm_params p) {
+// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.
+template<int SIZE, int KIND, int ITEMS>
+__global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : kNarrowBlocks / 2) layer_norm_narrow_kernel(const layer_norm_params p) {
     const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    float gamma[kNarrowItems][4], beta[kNarrowItems][4];
-    int col[kNarrowItems];
+    float gamma[ITEMS][4], beta[ITEMS][4];
+    int col[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kNarrowItems; ++i) {
-        col[i] = (i * p.lanes + in_row) * 4;
+    for (int i = 0; i < ITEMS; ++i) {
+        col[i] = min((i * p.lanes + in_row) * 4, p.columns);
         load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
         load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
     }
-    const float inverse = 1.0f / static_cast<float>(p.columns);
-    const std::int64_t warps = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32);
-    for (std::int64_t base = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp; base < p.rows;
-         base += warps * rows_per_warp) {
-        const std::int64_t row = base + group;
-        const bool active = row < p.rows;
-        raw_quad<SIZE> raw[kNarrowItems];
+    const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
+    const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
+    std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
+    raw_quad<SIZE> raw[ITEMS];
+    const auto fetch = [&](std::int64_t at) {
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             raw[i].clear();
-            if (active) raw[i].load(p.x.base + row * p.x.pitch, col[i], p.columns, p.per_access);
+            if (at < p.rows) raw[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
         }
-        float v[kNarrowItems][4], sum = 0.0f;
+    };
+    fetch(row);
+    for (; row - group < p.rows; row += step) {
+        float v[ITEMS][4], sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             raw[i].widen(half, v[i]);
             sum += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
         }
-        const float mean = lane_sum(sum, p.lanes) / static_cast<float>(p.columns); // a division: exact for rows of one value
+        fetch(row + step);
+        const float mean = lane_sum(sum, p.lanes) / count; // a division: exact for rows of one value
         float squares = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[i][k] -= mean;
-                if (held(col[i], k, p.columns, TAIL)) squares = fmaf(v[i][k], v[i][k], squares);
+            for (int k = 0; k < 4; ++k) v[i][k] -= mean;
+            if (col[i] + 4 > p.columns) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (col[i] + k >= p.columns) v[i][k] = 0.0f;
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) squares = fmaf(v[i][k], v[i][k], squares);
         }
         const float rstd = rsqrtf(lane_sum(squares, p.lanes) * inverse + p.epsilon);
-        if (!active) continue;
+        if (row >= p.rows) continue;
         if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             if (col[i] >= p.columns) continue;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = activation(fmaf(v[i][k] * rstd, gamma[i][k], beta[i][k]), p.epilogue);
+            for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(fmaf(v[i][k] * rstd, gamma[i][k], beta[i][k]));
             if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
             store_quad(p.y.base + row * p.y.pitch, col[i], p.columns, p.per_access, p.y.dtype, v[i]);
         }
     }
 }
 
-// A block or a cluster of blocks per row, each block with a slice of the columns; the next row's values are on their way while
-// this one's sums go round.
-template<int SIZE, int QT, bool CLUSTER>
-__global__ void __launch_bounds__(kWideThreads) layer_norm_wide_kernel(const layer_norm_params p) {
-    __shared__ wide_sums<1, CLUSTER> sums;
+// Rows of a step of a wide kernel.
+template<int SIZE, int QT>
+constexpr int kWideRows = (QT == 3 ? 8 : 4) / SIZE;
+
+// A block, or a cluster of blocks that take a slice of the columns each, works on R rows at a time.  Each warp takes the mean of
+// its columns and the squares of what differs from that; from all warps' numbers come the row's mean and variance,
+//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
+// with one exchange between them.  In a cluster the exchange of one step of rows goes round while the step before is written
+// and the one behind it is summed.
+template<int SIZE, int KIND, int QT, bool CLUSTER>
+__global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const layer_norm_params p) {
+    constexpr int R = kWideRows<SIZE, QT>;
+    __shared__ wide_notes<2 * R, CLUSTER> notes;
+    __shared__ float sizes[(CLUSTER ? kMostCluster : 1) * kMostWarps]; // columns of each warp
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, all_warps = p.cluster * warps;
     const int rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
-    const std::int64_t first = CLUSTER ? blockIdx.x / p.cluster : blockIdx.x, step = CLUSTER ? gridDim.x / p.cluster : gridDim.x;
+    const std::int64_t first = (CLUSTER ? blockIdx.x / p.cluster : blockIdx.x) * static_cast<std::int64_t>(R);
+    const std::int64_t stride = (CLUSTER ? gridDim.x / p.cluster : gridDim.x) * static_cast<std::int64_t>(R);
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
     float gamma[QT][4], beta[QT][4];
     int col[QT];
+    wide_columns<QT>(p, rank, col);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        const int quad = i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
-        col[i] = quad < p.slice_quads ? min((rank * p.slice_quads + quad) * 4, p.columns) : p.columns;
         load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
         load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
     }
-    const float inverse = 1.0f / static_cast<float>(p.columns);
-    raw_quad<SIZE> raw[QT];
+    const auto columns_of = [&](int w) { // of warp w of the block with this rank
+        return [&, w](int of_rank) {
+            int n = 0;
+            for (int i = 0; i < QT; ++i) {
+                const int begin = i * static_cast<int>(blockDim.x) + w * 32, end = min(begin + 32, p.slice_quads);
+                if (begin < end) n += max(0, min((of_rank * p.slice_quads + end) * 4, p.columns) - min((of_rank * p.slice_quads + begin) * 4, p.columns));
+            }
+            return n;
+        };
+    };
+    for (int i = threadIdx.x; i < all_warps; i += blockDim.x) sizes[i] = static_cast<float>(columns_of(i % warps)(i / warps));
+    const float size = static_cast<float>(columns_of(warp)(rank)), inverse_size = size > 0.0f ? 1.0f / size : 0.0f;
+    const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
+
+    raw_quad<SIZE> now[R][QT], next[R][QT], before[R][QT];
+    const auto fetch = [&](raw_quad<SIZE> (&raw)[R][QT], std::int64_t at) {
 #pragma unroll
-    for (int i = 0; i < QT; ++i) raw[i].load(p.x.base + first * p.x.pitch, col[i], p.columns, p.per_access);
-    if constexpr (CLUSTER) cluster_barrier(); // every block of the cluster has begun
-    for (std::int64_t row = first; row < p.rows; row += step) {
-        float v[QT][4], sum[1] = {0.0f};
+        for (int r = 0; r < R; ++r) {
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            raw[i].widen(half, v[i]);
-            sum[0] += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
-        }
-        if (row + step < p.rows) {
-#pragma unroll
-            for (int i = 0; i < QT; ++i) raw[i].load(p.x.base + (row + step) * p.x.pitch, col[i], p.columns, p.per_access);
-        }
-        sums.add_up(sum, 0, rank, p.cluster);
-        const float mean = sum[0] / static_cast<float>(p.columns);
-        sum[0] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[i][k] -= mean;
-                if (col[i] + k < p.columns) sum[0] = fmaf(v[i][k], v[i][k], sum[0]);
+            for (int i = 0; i < QT; ++i) {
+                raw[r][i].clear();
+                if (at + r < p.rows) raw[r][i].load(p.x.base + (at + r) * p.x.pitch, col[i], p.columns, p.per_access);
             }
         }
-        sums.add_up(sum, 1, rank, p.cluster);
-        const float rstd = rsqrtf(sum[0] * inverse + p.epsilon);
-        if (p.stats != nullptr && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+    };
+    // {sum, squares of what differs from the warp's mean} of each row
+    const auto summed = [&](float (&v)[2 * R]) {
+        float t[R];
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            if (col[i] >= p.columns) continue;
+        for (int r = 0; r < R; ++r) {
+            t[r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = activation(fmaf(v[i][k] * rstd, gamma[i][k], beta[i][k]), p.epilogue);
-            if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
-            store_quad(p.y.base + row * p.y.pitch, col[i], p.columns, p.per_access, p.y.dtype, v[i]);
+            for (int i = 0; i < QT; ++i) {
+                float x[4];
+                now[r][i].widen(half, x);
+                t[r] += (x[0] + x[1]) + (x[2] + x[3]);
+            }
+        }
+        warp_sums<R>(t);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            v[r] = t[r];
+            const float mean = t[r] * inverse_size;
+            t[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                float x[4];
+                now[r][i].widen(half, x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] -= mean;
+                if (col[i] + 4 > p.columns) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (col[i] + k >= p.columns) x[k] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) t[r] = fmaf(x[k], x[k], t[r]);
+            }
+        }
+        warp_sums<R>(t);
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[R + r] = t[r];
+    };
+    const auto finish = [&](const raw_quad<SIZE> (&raw)[R][QT], std::int64_t at, int set) {
+        float mean[R], var[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) mean[r] = var[r] = 0.0f;
+        for (int w = lane; w < all_warps; w += 32) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) mean[r] += notes.note[set][w][r];
+        }
+        warp_sums<R>(mean);
+#pragma unroll
+        for (int r = 0; r < R; ++r) mean[r] /= count; // exact for rows of one value
+        for (int w = lane; w < all_warps; w += 32) {
+            const float n = sizes[w], over = n > 0.0f ? 1.0f / n : 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float off = fmaf(notes.note[set][w][r], over, -mean[r]);
+                var[r] += fmaf(n * off, off, notes.note[set][w][R + r]);
+            }
+        }
+        warp_sums<R>(var);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const std::int64_t row = at + r;
+            if (row >= p.rows) break;
+            const float rstd = rsqrtf(var[r] * inverse + p.epsilon);
+            if (p.stats != nullptr && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean[r], rstd);
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                if (col[i] >= p.columns) continue;
+                float v[4];
+                raw[r][i].widen(half, v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = activation<KIND>(fmaf((v[k] - mean[r]) * rstd, gamma[i][k], beta[i][k]));
+                if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v);
+                store_quad(p.y.base + row * p.y.pitch, col[i], p.columns, p.per_access, p.y.dtype, v);
+            }
+        }
+    };
+
+    fetch(now, first);
+    int set = 0;
+    if constexpr (CLUSTER) {
+        cluster_arrive(); // every block of the cluster has begun
+        std::int64_t row = first;
+        for (; row < p.rows; row += stride) {
+            float v[2 * R];
+            summed(v);
+            cluster_wait();
+            notes.leave(v, set, rank, p.cluster);
+            cluster_arrive();
+            fetch(next, row + stride);
+            if (row != first) finish(before, row - stride, set == 0 ? 2 : set - 1);
+            set = next_set(set, 3);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i) {
+                    before[r][i] = now[r][i];
+                    now[r][i] = next[r][i];
+                }
+            }
+        }
+        cluster_wait();
+        if (row != first) finish(before, row - stride, set == 0 ? 2 : set - 1);
+    } else {
+        for (std::int64_t row = first; row < p.rows; row += stride, set ^= 1) {
+            float v[2 * R];
+            summed(v);
+            notes.leave(v, set, rank, p.cluster);
+            fetch(next, row + stride);
+            __syncthreads();
+            finish(now, row, set);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i) now[r][i] = next[r][i];
+            }
         }
     }
 }
 
-template<auto kernel>
+template<int SIZE, int KIND, int QT, bool CLUSTER>
 cb200_status launch_wide_forward(const layer_norm_params &p, const wide_shape &shape, int device, cudaStream_t stream) {
-    const std::int64_t clusters = std::min<std::int64_t>(p.rows, resident_clusters<kernel>(shape, device));
+    constexpr auto kernel = layer_norm_wide_kernel<SIZE, KIND, QT, CLUSTER>;
+    constexpr int step = kWideRows<SIZE, QT>;
+    const std::int64_t clusters = std::min<std::int64_t>((p.rows + step - 1) / step, resident_clusters<kernel>(shape, device));
     CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(clusters), stream));
     count_launch();
     return CB200_STATUS_SUCCESS;
 }
 
-template<int SIZE>
+template<int SIZE, int KIND>
 cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream) {
     if (p.columns <= kNarrowColumns) {
-        const std::int64_t per_block = kNarrowThreads / p.lanes;
-        const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>((p.rows + per_block - 1) / per_block, 148 * 4));
-        if (p.columns % 4 != 0) layer_norm_narrow_kernel<SIZE, true><<<grid, kNarrowThreads, 0, stream>>>(p);
-        else layer_norm_narrow_kernel<SIZE, false><<<grid, kNarrowThreads, 0, stream>>>(p);
+        const std::int64_t per_block = kNarrowThreads / p.lanes, blocks = (p.rows + per_block - 1) / per_block;
+        if (narrow_items(p.columns) == 2)
+            layer_norm_narrow_kernel<SIZE, KIND, 2><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
+        else
+            layer_norm_narrow_kernel<SIZE, KIND, 4><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks / 2)), kNarrowThreads, 0, stream>>>(p);
         count_launch();
         CB200_CUDA_OK(cudaGetLastError());
         return CB200_STATUS_SUCCESS;
@@ -146,9 +268,9 @@ cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream
     const wide_shape shape = wide_shape_of(p.columns);
     p.cluster = shape.cluster;
     p.slice_quads = shape.slice_quads;
-    if (shape.cluster == 1) return launch_wide_forward<layer_norm_wide_kernel<SIZE, 2, false>>(p, shape, device, stream);
-    if (shape.quads_per_thread == 2) return launch_wide_forward<layer_norm_wide_kernel<SIZE, 2, true>>(p, shape, device, stream);
-    return launch_wide_forward<layer_norm_wide_kernel<SIZE, 4, true>>(p, shape, device, stream);
+    if (shape.cluster == 1) return launch_wide_forward<SIZE, KIND, 3, false>(p, shape, device, stream);
+    if (shape.quads_per_thread == 3) return launch_wide_forward<SIZE, KIND, 3, true>(p, shape, device, stream);
+    return launch_wide_forward<SIZE, KIND, 4, true>(p, shape, device, stream);
 }
 
 } // namespace
@@ -167,5 +289,7 @@ extern "C" cb200_status cb200_layer_norm_forward(const cb200_layer_norm *d, void
     CB200_CUDA_OK(scope.status);
     if (p.rows == 0) return CB200_STATUS_SUCCESS;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return element_bytes(p.x.dtype) == 4 ? launch_forward<4>(p, d->device, s) : launch_forward<2>(p, d->device, s);
+    return with_epilogue(p.epilogue, [&](auto kind) {
+        return element_bytes(p.x.dtype) == 4 ? launch_forward<4, kind()>(p, d->device, s) : launch_forward<2, kind()>(p, d->device, s);
+    });
 }

@@ -717,7 +717,7 @@ cb200_status cb200_dropout_rows(const cb200_dropout_matrix *matrix, void *stream
 /* Layer norm over the columns of each row, with the activation and dropout that follow it in the same pass:
  *     u = (x - mean) / sqrt(var + epsilon),  z = gamma u + beta,  y = dropout(act(z)),
  * var the mean of the squared differences.  epilogue: CB200_EPILOGUE_NONE, _RELU, _GELU_ERF or _GELU_TANH (beta is the
- * bias).  1 to 65,536 columns, up to 2^32 rows; more are refused.
+ * bias).  1 to 65,536 columns, fewer than 2^32 rows; more are refused.
  * Forward writes y (which may be x, as for dropout) and, when asked, stats.
  * Backward reads x, dy and the stats of the forward call with the same parameters, epilogue and dropout, and writes
  * those of dx (which may be x or dy), dgamma and dbeta that are not NULL; relu's slope is 0 at 0.  It needs

@@ -10,8 +10,8 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # one value; less than a quad; a lane; several lanes, with and without a last piece of a quad; the widest row of a warp and the
-# first of a block; several warps; the first of a cluster of 2, of 4; the gene set; the first of four quads to a thread; the widest
-WIDTHS = [1, 2, 3, 4, 7, 16, 32, 50, 64, 100, 128, 255, 512, 513, 516, 1237, 4608, 4609, 9300, 33_538, 36_868, 65_536]
+# first of a block; several warps; the first of a cluster of 2, of 4, of 8; the gene set; the first of four quads to a thread; the widest
+WIDTHS = [1, 2, 3, 4, 7, 16, 32, 50, 64, 100, 128, 255, 512, 513, 516, 1237, 4608, 4609, 9300, 18_433, 33_538, 36_864, 36_868, 65_536]
 
 
 def rows_for(cols):
