@@ -14,45 +14,84 @@ struct dropout_params {
     row_matrix x, y;
     dropout_args drop;
     std::uint32_t rows;
-    std::uint32_t quads;                 // of a row
-    std::uint32_t step_rows, step_quads; // from one quad of a thread to its next
+    std::uint32_t pieces;                 // of a row: of Q quads each
+    std::uint32_t step_rows, step_pieces; // from one piece of a thread to its next
     int columns, per_access;
 };
 
-// A thread's quads lie a launch's width apart; it goes from one to the next by adding rows and quads, with no division.
-template<int SIZE>
+// A thread works on pieces of Q quads that lie a launch's width apart; it goes from one to the next by adding rows and pieces,
+// with no division.  Q = 2 for two-byte elements in rows of whole 16-byte pieces, where a piece is one load and one store.
+// WHOLE: rows are whole pieces and every access is aligned.
+template<int SIZE, int Q, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const dropout_params p) {
     const std::uint64_t first = static_cast<std::uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
     const std::uint64_t sequence = sequence_of(p.drop);
     const bool half = p.x.dtype == CB200_DTYPE_F16;
-    std::uint64_t row = first / p.quads;
-    std::uint32_t quad = static_cast<std::uint32_t>(first - row * p.quads);
+    std::uint64_t row = first / p.pieces;
+    std::uint32_t piece = static_cast<std::uint32_t>(first - row * p.pieces);
     while (row < p.rows) {
-        raw_quad<SIZE> raw[kInFlight];
-        std::uint32_t r[kInFlight], q[kInFlight];
+        raw_quad<SIZE> raw[kInFlight][Q];
+        std::uint32_t r[kInFlight], at[kInFlight];
         bool in[kInFlight];
 #pragma unroll
         for (int i = 0; i < kInFlight; ++i) {
             r[i] = static_cast<std::uint32_t>(row);
-            q[i] = quad;
+            at[i] = piece;
             in[i] = row < p.rows;
             row += p.step_rows;
-            quad += p.step_quads;
-            if (quad >= p.quads) {
-                quad -= p.quads;
+            piece += p.step_pieces;
+            if (piece >= p.pieces) {
+                piece -= p.pieces;
                 ++row;
             }
-            if (in[i]) raw[i].load(p.x.base + r[i] * p.x.pitch, static_cast<int>(q[i]) * 4, p.columns, p.per_access);
+            if (!in[i]) continue;
+            const unsigned char *x = p.x.base + r[i] * p.x.pitch;
+            if constexpr (WHOLE && Q == 2) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(x + static_cast<std::uint64_t>(at[i]) * 16u);
+                raw[i][0].w[0] = v.x; raw[i][0].w[1] = v.y; raw[i][1].w[0] = v.z; raw[i][1].w[1] = v.w;
+            } else if constexpr (WHOLE) {
+                raw[i][0].template load<4>(x + static_cast<std::uint64_t>(at[i]) * (4u * SIZE), 4);
+            } else {
+                const int col[1] = {static_cast<int>(at[i]) * 4};
+                load_quads<SIZE, 1>(x, col, p.columns, p.per_access, raw[i]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kInFlight; ++i) {
             if (!in[i]) break;
-            float v[4];
-            raw[i].widen(half, v);
-            if (p.drop.on) drop_quad(p.drop, sequence, r[i], q[i], v);
-            store_quad(p.y.base + r[i] * p.y.pitch, static_cast<int>(q[i]) * 4, p.columns, p.per_access, p.y.dtype, v);
+            float v[Q][4];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                raw[i][q].widen(half, v[q]);
+                if (p.drop.on) drop_quad(p.drop, sequence, r[i], at[i] * Q + q, v[q]);
+            }
+            unsigned char *y = p.y.base + r[i] * p.y.pitch;
+            if constexpr (WHOLE && Q == 2) { // a result of two bytes as well
+                const bool y_half = p.y.dtype == CB200_DTYPE_F16;
+                *reinterpret_cast<uint4 *>(y + static_cast<std::uint64_t>(at[i]) * 16u) =
+                    make_uint4(pack_pair(v[0][0], v[0][1], y_half), pack_pair(v[0][2], v[0][3], y_half), pack_pair(v[1][0], v[1][1], y_half),
+                               pack_pair(v[1][2], v[1][3], y_half));
+            } else {
+                const int col[1] = {static_cast<int>(at[i]) * 4};
+                store_quads<1>(y, col, p.columns, WHOLE ? 4 : p.per_access, p.y.dtype, v);
+            }
         }
     }
+}
+
+template<int SIZE, int Q, bool WHOLE>
+cb200_status launch(dropout_params p, std::int64_t rows, cudaStream_t stream) {
+    p.rows = static_cast<std::uint32_t>(rows);
+    p.pieces = static_cast<std::uint32_t>((p.columns + 4ll * Q - 1) / (4 * Q));
+    const std::int64_t threads = (rows * static_cast<std::int64_t>(p.pieces) + kInFlight - 1) / kInFlight;
+    const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>((threads + kThreads - 1) / kThreads, 148 * 8));
+    const std::int64_t step = static_cast<std::int64_t>(grid) * kThreads;
+    p.step_rows = static_cast<std::uint32_t>(step / p.pieces);
+    p.step_pieces = static_cast<std::uint32_t>(step % p.pieces);
+    dropout_kernel<SIZE, Q, WHOLE><<<grid, kThreads, 0, stream>>>(p);
+    count_launch();
+    CB200_CUDA_OK(cudaGetLastError());
+    return CB200_STATUS_SUCCESS;
 }
 
 } // namespace
@@ -74,19 +113,12 @@ extern "C" cb200_status cb200_dropout_rows(const cb200_dropout_matrix *m, void *
     device_scope scope(m->device);
     CB200_CUDA_OK(scope.status);
     if (m->rows == 0 || m->columns == 0) return CB200_STATUS_SUCCESS;
-    p.rows = static_cast<std::uint32_t>(m->rows);
     p.columns = static_cast<int>(m->columns);
-    p.quads = static_cast<std::uint32_t>((m->columns + 3) / 4);
-    p.per_access = columns_per_access(p.y, columns_per_access(p.x, 4));
-    const std::int64_t threads = (m->rows * static_cast<std::int64_t>(p.quads) + kInFlight - 1) / kInFlight;
-    const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>((threads + kThreads - 1) / kThreads, 148 * 8));
-    const std::int64_t step = static_cast<std::int64_t>(grid) * kThreads;
-    p.step_rows = static_cast<std::uint32_t>(step / p.quads);
-    p.step_quads = static_cast<std::uint32_t>(step % p.quads);
+    p.per_access = columns_per_access(p.y, columns_per_access(p.x, columns_of_access(m->columns)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (element_bytes(p.x.dtype) == 4) dropout_kernel<4><<<grid, kThreads, 0, s>>>(p);
-    else dropout_kernel<2><<<grid, kThreads, 0, s>>>(p);
-    count_launch();
-    CB200_CUDA_OK(cudaGetLastError());
-    return CB200_STATUS_SUCCESS;
+    const bool whole = p.per_access == 4;
+    if (element_bytes(p.x.dtype) == 4) return whole ? launch<4, 1, true>(p, m->rows, s) : launch<4, 1, false>(p, m->rows, s);
+    if (whole && element_bytes(p.y.dtype) == 2 && p.columns % 8 == 0 && columns_per_access(p.x, 8) == 8 && columns_per_access(p.y, 8) == 8)
+        return launch<2, 2, true>(p, m->rows, s);
+    return whole ? launch<2, 1, true>(p, m->rows, s) : launch<2, 1, false>(p, m->rows, s);
 }

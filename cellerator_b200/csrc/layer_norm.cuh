@@ -16,6 +16,7 @@ namespace cb200 {
 constexpr int kNarrowColumns = 512;
 constexpr std::int64_t kMostColumns = 65536;
 constexpr int kNarrowThreads = 256;
+constexpr int kNarrowItems = 4; // quads of a row that a lane holds
 // Most threads of a block of a wide row, by the quads of a thread.  Three quads and twelve warps: three warps to a scheduler leave
 // each thread 168 registers, and eight such blocks hold 36,864 columns.
 constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 3 ? 384 : 512; }
@@ -108,13 +109,11 @@ unsigned resident_clusters(const wide_shape &shape, int device) {
     return static_cast<unsigned>(found);
 }
 
-// A narrow row: quads that a lane holds, and lanes of the row, as few as hold it (its sums then take few shuffles).  Two quads
-// up to 256 columns, so that the backward pass, which keeps four numbers a column, has room for 24 warps an SM.
-inline int narrow_items(std::int64_t columns) { return columns <= 256 ? 2 : 4; }
-inline int narrow_lanes(std::int64_t columns) {
+// Lanes of a narrow row, with `items` quads to a lane: as few as hold it, so that its sums take few shuffles.
+inline int narrow_lanes(std::int64_t columns, int items) {
     const std::int64_t quads = (columns + 3) / 4;
     int lanes = 1;
-    while (lanes < 32 && lanes * narrow_items(columns) < quads) lanes *= 2;
+    while (lanes < 32 && lanes * items < quads) lanes *= 2;
     return lanes;
 }
 
@@ -141,8 +140,8 @@ inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward,
     p->columns = static_cast<int>(d->columns);
     p->epilogue = d->epilogue;
     p->epsilon = d->epsilon;
-    p->lanes = narrow_lanes(d->columns);
-    p->per_access = columns_per_access(p->x, 4);
+    p->lanes = narrow_lanes(d->columns, kNarrowItems);
+    p->per_access = columns_per_access(p->x, columns_of_access(d->columns));
     if (!backward && !(d->epsilon >= 0.0f && d->epsilon < 3.4e38f)) return fail(CB200_STATUS_INVALID_ARGUMENT, "epsilon %g is no number from 0 on", d->epsilon);
     return CB200_STATUS_SUCCESS;
 }
@@ -165,9 +164,20 @@ __device__ __forceinline__ void load_parameters(const float *v, int col, int n, 
     for (int k = 0; k < 4; ++k) out[k] = v != nullptr && col + k < n ? __ldg(v + col + k) : otherwise;
 }
 
-// Logistic function: 1 / (1 + e^-t), within a few units of the last place of 1 (the exponential's argument keeps 2^-24 of
-// itself).
-__device__ __forceinline__ float logistic(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
+// e^t and 1 / t by the hardware's approximations: e^t within 2 + 1.2 |t| units of the last place, 1 / t within one; what is too
+// small for a normal number is 0.
+__device__ __forceinline__ float fast_exp(float t) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t * 1.4426950408889634f));
+    return e;
+}
+__device__ __forceinline__ float fast_reciprocal(float t) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+    return r;
+}
+// Logistic function: 1 / (1 + e^-t), within a few units of the last place of 1.
+__device__ __forceinline__ float logistic(float t) { return fast_reciprocal(1.0f + fast_exp(-t)); }
 
 // act(z).  The tanh form of GELU, z / 2 (1 + tanh(c (z + 0.044715 z^3))), is z times the logistic function of twice that argument.
 template<int KIND>
@@ -183,7 +193,7 @@ template<int KIND>
 __device__ __forceinline__ float through_activation(float dy, float z) {
     if constexpr (KIND == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
     if constexpr (KIND == CB200_EPILOGUE_GELU_ERF)
-        return dy * fmaf(z, 0.39894228040143268f * __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+        return dy * fmaf(z, 0.39894228040143268f * fast_exp(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
     if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) {
         const float zz = z * z, gate = logistic(1.5957691216057308f * z * fmaf(0.044715f, zz, 1.0f));
         const float steep = gate * (1.0f - gate); // 0 far from 0, where the polynomial may be infinite
@@ -192,10 +202,15 @@ __device__ __forceinline__ float through_activation(float dy, float z) {
     return dy;
 }
 
-// Sum over groups of `lanes` neighbouring lanes, in each of them.
-__device__ __forceinline__ float lane_sum(float v, int lanes) {
-    for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
+// Sums over groups of `lanes` neighbouring lanes (a power of two), in each of them.
+template<int N>
+__device__ __forceinline__ void lane_sums(float (&v)[N], int lanes) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        if (off >= lanes) break;
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+    }
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }

@@ -10,6 +10,8 @@ namespace cb200 {
 namespace {
 
 // Most blocks (narrow) or clusters (wide) of a launch: each leaves 2 x columns sums.
+// Quads of a row that a lane holds: two up to 256 columns, as it keeps two sums for each of its columns and 24 warps are to fit an SM.
+constexpr int back_items(std::int64_t columns) { return columns <= 256 ? 2 : 4; }
 constexpr int kNarrowBlocks = 3; // narrow: resident on an SM, with two quads a lane; one less with four
 constexpr int kNarrowParts = 148 * kNarrowBlocks;
 constexpr int kWideParts = 148 * 4;
@@ -63,16 +65,10 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
     raw_quad<SG> raw_dy[ITEMS];
     float2 stats = make_float2(0.0f, 0.0f);
     const auto fetch = [&](std::int64_t at) {
-        if (at < p.rows) stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            raw_x[i].clear();
-            raw_dy[i].clear();
-            if (at < p.rows) {
-                raw_x[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
-                raw_dy[i].load(p.dy.base + at * p.dy.pitch, col[i], p.columns, p.per_access);
-            }
-        }
+        if (at >= p.rows) return;
+        stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
+        load_quads(p.x.base + at * p.x.pitch, col, p.columns, p.per_access, raw_x);
+        load_quads(p.dy.base + at * p.dy.pitch, col, p.columns, p.per_access, raw_dy);
     };
     fetch(row);
     for (; row - group < p.rows; row += step) {
@@ -94,16 +90,16 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
             if constexpr (KIND != CB200_EPILOGUE_NONE) *reinterpret_cast<float4 *>(beta) = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
             terms.apply(x[i], dy[i], gamma, beta, dgamma[i], dbeta[i], sums);
         }
-        sums[0] = lane_sum(sums[0], p.lanes) * inverse;
-        sums[1] = lane_sum(sums[1], p.lanes) * inverse;
+        lane_sums(sums, p.lanes);
+        sums[0] *= inverse;
+        sums[1] *= inverse;
         if (!active || p.dx.base == nullptr) continue;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            if (col[i] >= p.columns) continue;
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[i][k] = terms.rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
-            store_quad(p.dx.base + row * p.dx.pitch, col[i], p.columns, p.per_access, p.dx.dtype, x[i]);
         }
+        store_quads(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, x);
     }
     let_next_launch_start();
     if (p.partials == nullptr) return;
@@ -158,11 +154,8 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(
     const auto fetch = [&](std::int64_t at) {
         if (at >= p.rows) return;
         stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            raw_x[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
-            raw_dy[i].load(p.dy.base + at * p.dy.pitch, col[i], p.columns, p.per_access);
-        }
+        load_quads(p.x.base + at * p.x.pitch, col, p.columns, p.per_access, raw_x);
+        load_quads(p.dy.base + at * p.dy.pitch, col, p.columns, p.per_access, raw_dy);
     };
     float x[QT][4], dy[QT][4]; // x and dy of a row, then its u and h
     const auto widened = [&]() {
@@ -193,14 +186,13 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(
         warp_sums<2>(sums);
         sums[0] *= inverse;
         sums[1] *= inverse;
+        float v[QT][4];
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-            if (col[i] >= p.columns) continue;
-            float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = rstd * (h[i][k] - sums[0] - u[i][k] * sums[1]);
-            store_quad(p.dx.base + row * p.dx.pitch, col[i], p.columns, p.per_access, p.dx.dtype, v);
+            for (int k = 0; k < 4; ++k) v[i][k] = rstd * (h[i][k] - sums[0] - u[i][k] * sums[1]);
         }
+        store_quads(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, v);
     };
     fetch(first);
     int set = 0;
@@ -279,8 +271,8 @@ __global__ void __launch_bounds__(kMeetWarps * 32) layer_norm_meet_kernel(const 
 
 // Blocks of a launch over narrow rows.
 std::int64_t narrow_parts(std::int64_t rows, std::int64_t columns) {
-    const std::int64_t per_block = kNarrowThreads / narrow_lanes(columns);
-    return std::min<std::int64_t>((rows + per_block - 1) / per_block, narrow_items(columns) == 2 ? kNarrowParts : kNarrowParts / kNarrowBlocks * (kNarrowBlocks - 1));
+    const std::int64_t per_block = kNarrowThreads / narrow_lanes(columns, back_items(columns));
+    return std::min<std::int64_t>((rows + per_block - 1) / per_block, back_items(columns) == 2 ? kNarrowParts : kNarrowParts / kNarrowBlocks * (kNarrowBlocks - 1));
 }
 
 struct backward_launch {
@@ -308,7 +300,8 @@ struct backward_launch {
     cb200_status run() {
         if (p.columns <= kNarrowColumns) {
             const std::int64_t parts = narrow_parts(p.rows, p.columns);
-            if (narrow_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            p.lanes = narrow_lanes(p.columns, back_items(p.columns));
+            if (back_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             else layer_norm_back_narrow_kernel<SX, SG, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             return finish(parts);
         }

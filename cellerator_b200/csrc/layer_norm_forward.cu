@@ -7,46 +7,44 @@
 namespace cb200 {
 namespace {
 
-constexpr int kNarrowBlocks = 4; // resident on an SM
+constexpr int kNarrowBlocks = 3; // resident on an SM
 
-// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.
-template<int SIZE, int KIND, int ITEMS>
-__global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : kNarrowBlocks / 2) layer_norm_narrow_kernel(const layer_norm_params p) {
+// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
+// shared memory: a lane's sixteen columns of them would take a third of its registers.
+template<int SIZE, int KIND>
+__global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narrow_kernel(const layer_norm_params p) {
+    __shared__ __align__(16) float parameters[2][kNarrowColumns];
     const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
-    const bool half = p.x.dtype == CB200_DTYPE_F16;
+    const bool half = p.x.dtype == CB200_DTYPE_F16, affine = p.gamma != nullptr || p.beta != nullptr;
     const std::uint64_t sequence = sequence_of(p.drop);
-    float gamma[ITEMS][4], beta[ITEMS][4];
-    int col[ITEMS];
+    int col[kNarrowItems];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        col[i] = min((i * p.lanes + in_row) * 4, p.columns);
-        load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
-        load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
-    }
+    for (int i = 0; i < kNarrowItems; ++i) col[i] = min((i * p.lanes + in_row) * 4, p.columns);
     const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
     std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
-    raw_quad<SIZE> raw[ITEMS];
-    const auto fetch = [&](std::int64_t at) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            raw[i].clear();
-            if (at < p.rows) raw[i].load(p.x.base + at * p.x.pitch, col[i], p.columns, p.per_access);
+    raw_quad<SIZE> raw[kNarrowItems];
+    if (row < p.rows) load_quads(p.x.base + row * p.x.pitch, col, p.columns, p.per_access, raw);
+    if (affine) {
+        for (int c = threadIdx.x; c < kNarrowColumns; c += kNarrowThreads) {
+            parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
+            parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
         }
-    };
-    fetch(row);
+        __syncthreads();
+    }
     for (; row - group < p.rows; row += step) {
-        float v[ITEMS][4], sum = 0.0f;
+        float v[kNarrowItems][4], sum[1] = {0.0f};
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
+        for (int i = 0; i < kNarrowItems; ++i) {
             raw[i].widen(half, v[i]);
-            sum += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+            sum[0] += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
         }
-        fetch(row + step);
-        const float mean = lane_sum(sum, p.lanes) / count; // a division: exact for rows of one value
-        float squares = 0.0f;
+        if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
+        lane_sums(sum, p.lanes);
+        const float mean = sum[0] / count; // a division: exact for rows of one value
+        sum[0] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
+        for (int i = 0; i < kNarrowItems; ++i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[i][k] -= mean;
             if (col[i] + 4 > p.columns) {
@@ -55,19 +53,28 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
                     if (col[i] + k >= p.columns) v[i][k] = 0.0f;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) squares = fmaf(v[i][k], v[i][k], squares);
+            for (int k = 0; k < 4; ++k) sum[0] = fmaf(v[i][k], v[i][k], sum[0]);
         }
-        const float rstd = rsqrtf(lane_sum(squares, p.lanes) * inverse + p.epsilon);
+        lane_sums(sum, p.lanes);
+        const float rstd = rsqrtf(fmaf(sum[0], inverse, p.epsilon));
         if (row >= p.rows) continue;
         if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
+        for (int i = 0; i < kNarrowItems; ++i) {
             if (col[i] >= p.columns) continue;
+            if (affine) {
+                const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
+                v[i][0] = activation<KIND>(fmaf(v[i][0] * rstd, g.x, b.x));
+                v[i][1] = activation<KIND>(fmaf(v[i][1] * rstd, g.y, b.y));
+                v[i][2] = activation<KIND>(fmaf(v[i][2] * rstd, g.z, b.z));
+                v[i][3] = activation<KIND>(fmaf(v[i][3] * rstd, g.w, b.w));
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(fmaf(v[i][k] * rstd, gamma[i][k], beta[i][k]));
+                for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(v[i][k] * rstd);
+            }
             if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
-            store_quad(p.y.base + row * p.y.pitch, col[i], p.columns, p.per_access, p.y.dtype, v[i]);
         }
+        store_quads(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
     }
 }
 
@@ -117,11 +124,7 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
     const auto fetch = [&](raw_quad<SIZE> (&raw)[R][QT], std::int64_t at) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                raw[r][i].clear();
-                if (at + r < p.rows) raw[r][i].load(p.x.base + (at + r) * p.x.pitch, col[i], p.columns, p.per_access);
-            }
+            if (at + r < p.rows) load_quads(p.x.base + (at + r) * p.x.pitch, col, p.columns, p.per_access, raw[r]);
         }
     };
     // {sum, squares of what differs from the warp's mean} of each row
@@ -188,16 +191,15 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
             if (row >= p.rows) break;
             const float rstd = rsqrtf(var[r] * inverse + p.epsilon);
             if (p.stats != nullptr && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean[r], rstd);
+            float v[QT][4];
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
-                if (col[i] >= p.columns) continue;
-                float v[4];
-                raw[r][i].widen(half, v);
+                raw[r][i].widen(half, v[i]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = activation<KIND>(fmaf((v[k] - mean[r]) * rstd, gamma[i][k], beta[i][k]));
-                if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v);
-                store_quad(p.y.base + row * p.y.pitch, col[i], p.columns, p.per_access, p.y.dtype, v);
+                for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(fmaf((v[i][k] - mean[r]) * rstd, gamma[i][k], beta[i][k]));
+                if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
             }
+            store_quads(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
         }
     };
 
@@ -257,10 +259,7 @@ template<int SIZE, int KIND>
 cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream) {
     if (p.columns <= kNarrowColumns) {
         const std::int64_t per_block = kNarrowThreads / p.lanes, blocks = (p.rows + per_block - 1) / per_block;
-        if (narrow_items(p.columns) == 2)
-            layer_norm_narrow_kernel<SIZE, KIND, 2><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
-        else
-            layer_norm_narrow_kernel<SIZE, KIND, 4><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks / 2)), kNarrowThreads, 0, stream>>>(p);
+        layer_norm_narrow_kernel<SIZE, KIND><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
         count_launch();
         CB200_CUDA_OK(cudaGetLastError());
         return CB200_STATUS_SUCCESS;

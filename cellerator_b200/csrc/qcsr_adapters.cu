@@ -5,15 +5,19 @@
 #include "kernels.cuh"
 
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 namespace cb200 {
 namespace {
 
-constexpr int kSegment = 128;   // entries that a warp decodes at a time
-constexpr int kMostParts = 32;  // of a row
-constexpr int kMostWarps = 8;
+constexpr int kRuns = 4;                // runs of 32 entries that a warp decodes at a time
+constexpr int kSegment = 32 * kRuns;
+constexpr int kMostParts = 32;          // of a row
+constexpr int kWarps = 8;
+constexpr int kMostRows = 8;            // of a block
 constexpr int kMostRank = 256;
+constexpr int kSumsBytes = 32 * 1024;   // of parts' sums in shared memory, or one row's
 
 struct adapter_params {
     const std::int64_t *row_ptr, *packed_row_ptr;
@@ -26,10 +30,11 @@ struct adapter_params {
     const float *scale;
     float *out;
     const float *bias;
-    std::int64_t row_begin, cols, adapters, out_ld, n;
+    std::int64_t row_begin, row_end, cols, adapters, out_ld, n;
     float alpha, beta;
     int rank, policy, epilogue;
-    int lanes; // that serve an entry: a power of two
+    int lanes;      // that serve an entry: a power of two
+    int block_rows; // rows of a block
 };
 
 // Entries of a part of a row of `len` entries, a multiple of a warp's segment: by the length alone.
@@ -42,10 +47,11 @@ __device__ __forceinline__ std::int64_t part_entries(std::int64_t len) {
 template<typename WT, int V>
 struct slice {
     static constexpr int bytes = V * static_cast<int>(sizeof(WT));
-    std::uint32_t w[bytes >= 4 ? bytes / 4 : 1];
+    static constexpr int words = bytes >= 4 ? bytes / 4 : 1;
+    std::uint32_t w[words];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < (bytes >= 4 ? bytes / 4 : 1); ++i) w[i] = 0u;
+        for (int i = 0; i < words; ++i) w[i] = 0u;
     }
     __device__ __forceinline__ void load(const unsigned char *p) {
         if constexpr (bytes == 16) {
@@ -60,123 +66,186 @@ struct slice {
             w[0] = __ldg(reinterpret_cast<const unsigned short *>(p));
         }
     }
+    // acc += v * w; pairs of columns with the two-wide fp32 FMA
     __device__ __forceinline__ void add_to(float (&acc)[V], float v) const {
         if constexpr (V == 1) {
             acc[0] = fmaf(v, __uint_as_float(sizeof(WT) == 2 ? w[0] << 16 : w[0]), acc[0]);
         } else {
+            const float2 vv = make_float2(v, v);
+            unsigned long long vp;
+            memcpy(&vp, &vv, 8);
 #pragma unroll
             for (int i = 0; i < V; i += 2) {
-                float a, b;
-                if constexpr (sizeof(WT) == 2) bf16x2_to_f32(w[i / 2], a, b);
-                else { a = __uint_as_float(w[i]); b = __uint_as_float(w[i + 1]); }
-                acc[i] = fmaf(v, a, acc[i]);
-                acc[i + 1] = fmaf(v, b, acc[i + 1]);
+                float2 f;
+                if constexpr (sizeof(WT) == 2) bf16x2_to_f32(w[i / 2], f.x, f.y);
+                else f = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+                float2 a = make_float2(acc[i], acc[i + 1]);
+                unsigned long long ap, fp;
+                memcpy(&ap, &a, 8);
+                memcpy(&fp, &f, 8);
+                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(ap) : "l"(vp), "l"(fp));
+                memcpy(&a, &ap, 8);
+                acc[i] = a.x;
+                acc[i + 1] = a.y;
             }
         }
     }
 };
 
-// A block per row.  Its warps take the row's parts in turn; a warp decodes 128 entries at a time into shared memory, {gene,
-// value}, and then `lanes` lanes serve an entry, V columns of A each.
+// A block takes p.block_rows rows, cut into parts by their lengths alone, and deals the parts to its warps, so that a long row
+// does not hold up the others.  A warp decodes 128 entries at a time into shared memory, {gene, value}, the next ones' indices and
+// codes being on their way meanwhile; then `lanes` lanes serve an entry, V columns of A each, 8 rows of A in flight.  A part's sum is
+// that of 32 / lanes classes of its entries, a row's that of its parts in order, and the product with B follows from shared memory.
 template<int BITS, typename WT, int V>
-__global__ void __launch_bounds__(kMostWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
-    __shared__ __align__(16) int2 staged[kMostWarps][kSegment];
-    __shared__ float hidden[kMostRank];
+__global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
+    __shared__ __align__(16) int2 staged[kWarps][kSegment];
+    __shared__ std::int64_t row_start[kMostRows], code_start[kMostRows], row_len[kMostRows], row_share[kMostRows];
+    __shared__ int row_adapter[kMostRows], first_part[kMostRows + 1];
     extern __shared__ float sums[]; // [parts][rank]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const std::int64_t row = p.row_begin + blockIdx.x;
-    const int a = __ldg(p.adapter + row);
-    const bool has = a >= 0 && a < p.adapters;
-    if (has) {
-        const std::int64_t start = __ldg(p.row_ptr + row), len = __ldg(p.row_ptr + row + 1) - start;
-        const std::int64_t share = part_entries(len);
-        const int parts = static_cast<int>((len + share - 1) / share);
-        const std::int32_t *cols = p.col_idx + start;
-        const std::uint8_t *codes = p.packed + (p.packed_row_ptr != nullptr ? __ldg(p.packed_row_ptr + row) : start);
-        const bool row_policy = p.policy == CB200_DECODE_COLUMN_SCALE_ROW_OFFSET;
-        const float row_offset = row_policy && p.offsets != nullptr ? __ldg(p.offsets + row) : 0.0f;
-        const int lanes = p.lanes, groups = 32 / lanes, group = lane / lanes, in_row = lane & (lanes - 1);
-        const unsigned row_bytes = static_cast<unsigned>(p.rank) * sizeof(WT);
-        const unsigned char *down = p.down + static_cast<std::int64_t>(a) * p.cols * row_bytes;
-        for (int part = warp; part < parts; part += warps) {
-            for (int first = 0; first < p.rank; first += lanes * V) { // columns of A; one turn but for wide ranks of narrow slices
-                const int col = first + in_row * V;
-                const bool holds = col < p.rank;
-                float acc[V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const std::int64_t row0 = p.row_begin + static_cast<std::int64_t>(blockIdx.x) * p.block_rows;
+    const int rows = static_cast<int>(min(static_cast<std::int64_t>(p.block_rows), p.row_end - row0));
+    if (warp == 0) {
+        int upto = 0;
+        if (lane < rows) {
+            const int a = __ldg(p.adapter + row0 + lane);
+            const bool has = a >= 0 && a < p.adapters;
+            const std::int64_t start = __ldg(p.row_ptr + row0 + lane), len = has ? __ldg(p.row_ptr + row0 + lane + 1) - start : 0, share = part_entries(len);
+            row_adapter[lane] = has ? a : -1;
+            row_start[lane] = start;
+            row_len[lane] = len;
+            row_share[lane] = share;
+            code_start[lane] = p.packed_row_ptr != nullptr ? __ldg(p.packed_row_ptr + row0 + lane) : start;
+            upto = static_cast<int>((len + share - 1) / share);
+        }
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-                const std::int64_t to = min(len, (part + 1) * share);
-                for (std::int64_t at = part * share; at < to; at += kSegment) {
+        for (int off = 1; off < kMostRows; off <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += below;
+        }
+        if (lane == 0) first_part[0] = 0;
+        if (lane < rows) first_part[lane + 1] = upto;
+    }
+    __syncthreads();
+    const int parts = first_part[rows];
+    const bool row_policy = p.policy == CB200_DECODE_COLUMN_SCALE_ROW_OFFSET;
+    const int lanes = p.lanes, groups = 32 / lanes, group = lane / lanes, in_row = lane & (lanes - 1);
+    const unsigned row_bytes = static_cast<unsigned>(p.rank) * sizeof(WT);
+    int2 *stage = staged[warp];
+    for (int column0 = 0; column0 < p.rank; column0 += lanes * V) { // of A; one turn but for wide ranks of narrow slices
+        const int col = column0 + in_row * V;
+        const bool holds = col < p.rank;
+        int part = warp, r = 0, gene[kRuns];
+        unsigned code[kRuns];
+        std::int64_t at = 0, to = 0; // entries of row r: those of the segment start at `at`
+        const auto fetch = [&]() {
+            const std::int32_t *cols = p.col_idx + row_start[r];
+            const std::uint8_t *codes = p.packed + code_start[r];
 #pragma unroll
-                    for (int i = 0; i < kSegment / 32; ++i) {
-                        const std::int64_t e = at + i * 32 + lane;
-                        int2 entry = make_int2(-1, 0);
-                        if (e < to) {
-                            const std::int32_t gene = __ldg(cols + e);
-                            unsigned code;
-                            if constexpr (BITS == 8) code = __ldg(codes + e);
-                            else code = (__ldg(codes + (e >> 1)) >> (4 * (e & 1))) & 15u;
-                            if (gene >= 0 && gene < p.cols) {
-                                const float scale = p.scales != nullptr ? __ldg(p.scales + gene) : 1.0f;
-                                const float offset = row_policy ? row_offset : p.offsets != nullptr ? __ldg(p.offsets + gene) : 0.0f;
-                                entry = make_int2(gene, __float_as_int(fmaf(static_cast<float>(code), scale, offset)));
-                            }
-                        }
-                        staged[warp][i * 32 + lane] = entry;
-                    }
-                    __syncwarp();
-                    const int count = static_cast<int>(min(static_cast<std::int64_t>(kSegment), to - at));
-                    for (int e = group; e < count + group; e += 4 * groups) {
-                        slice<WT, V> w[4];
-                        float v[4];
+            for (int i = 0; i < kRuns; ++i) {
+                const std::int64_t e = at + i * 32 + lane;
+                gene[i] = -1;
+                code[i] = 0u;
+                if (e >= to) continue;
+                gene[i] = __ldg(cols + e);
+                if constexpr (BITS == 8) code[i] = __ldg(codes + e);
+                else code[i] = (__ldg(codes + (e >> 1)) >> (4 * (e & 1))) & 15u;
+            }
+        };
+        const auto open = [&]() {
+            if (part >= parts) return;
+            r = __popc(__ballot_sync(0xffffffffu, lane < rows && first_part[min(lane, kMostRows)] <= part)) - 1;
+            at = (part - first_part[r]) * row_share[r];
+            to = min(row_len[r], at + row_share[r]);
+            fetch();
+        };
+        open();
+        float acc[V];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int2 entry = e + u * groups < kSegment ? staged[warp][e + u * groups] : make_int2(-1, 0);
-                            v[u] = __int_as_float(entry.y);
-                            w[u].clear();
-                            if (entry.x >= 0 && holds) w[u].load(down + static_cast<std::uint64_t>(entry.x) * row_bytes + col * sizeof(WT));
-                        }
+        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+        while (part < parts) {
+            const float row_offset = row_policy && p.offsets != nullptr ? __ldg(p.offsets + row0 + r) : 0.0f;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) w[u].add_to(acc, v[u]);
-                    }
-                    __syncwarp();
+            for (int i = 0; i < kRuns; ++i) {
+                int2 entry = make_int2(-1, 0); // what is left out, and what lies behind the part's end
+                if (gene[i] >= 0 && gene[i] < p.cols) {
+                    const float scale = p.scales != nullptr ? __ldg(p.scales + gene[i]) : 1.0f;
+                    const float offset = row_policy ? row_offset : p.offsets != nullptr ? __ldg(p.offsets + gene[i]) : 0.0f;
+                    entry = make_int2(gene[i], __float_as_int(fmaf(static_cast<float>(code[i]), scale, offset)));
+                }
+                stage[i * 32 + lane] = entry;
+            }
+            __syncwarp();
+            const unsigned char *down = p.down + static_cast<std::int64_t>(row_adapter[r]) * p.cols * row_bytes + col * sizeof(WT);
+            const int count = static_cast<int>(min(static_cast<std::int64_t>(kSegment), to - at)), part_now = part;
+            at += kSegment;
+            const bool ends = at >= to;
+            if (ends) {
+                part += kWarps;
+                open();
+            } else {
+                fetch();
+            }
+            const auto add = [&](auto unrolled, int e) {
+                constexpr int U = decltype(unrolled)::value;
+                slice<WT, V> w[U];
+                float v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int2 entry = stage[e + u * groups];
+                    v[u] = __int_as_float(entry.y);
+                    w[u].clear();
+                    if (entry.x >= 0 && holds) w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(entry.x)) * row_bytes);
                 }
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    for (int off = lanes; off < 32; off <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
-                    if (group == 0 && col + i < p.rank) sums[part * p.rank + col + i] = acc[i];
-                }
+                for (int u = 0; u < U; ++u) w[u].add_to(acc, v[u]);
+            };
+            // 128 / groups turns, 4 at least
+            int e = 0;
+            for (; e + 8 * groups <= kSegment && e < count; e += 8 * groups) add(std::integral_constant<int, 8>{}, e + group);
+            if (e < count) add(std::integral_constant<int, 4>{}, e + group); // 32 groups: one entry to a lane
+            __syncwarp();
+            if (!ends) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                for (int off = lanes; off < 32; off <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
+                if (group == 0 && col + i < p.rank) sums[part_now * p.rank + col + i] = acc[i];
+                acc[i] = 0.0f;
             }
         }
-        __syncthreads();
-        for (int k = threadIdx.x; k < p.rank; k += blockDim.x) {
-            float h = 0.0f;
-            for (int part = 0; part < parts; ++part) h += sums[part * p.rank + k];
-            hidden[k] = h;
-        }
-        __syncthreads();
     }
-    const float factor = has ? p.alpha * (p.scale != nullptr ? __ldg(p.scale + a) : 1.0f) : 0.0f;
-    const WT *up = static_cast<const WT *>(p.up) + static_cast<std::int64_t>(has ? a : 0) * p.rank * p.n;
-    for (std::int64_t c = threadIdx.x; c < p.n; c += blockDim.x) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * p.rank; i += kWarps * 32) {
+        const int r = i / p.rank, k = i - r * p.rank, last = first_part[r + 1];
+        if (first_part[r] == last) continue;
+        float *sum = sums + first_part[r] * p.rank + k, h = *sum;
+        for (int part = first_part[r] + 1; part < last; ++part) h += sums[part * p.rank + k];
+        *sum = h;
+    }
+    __syncthreads();
+    const int n = static_cast<int>(p.n);
+    for (int i = threadIdx.x; i < rows * n; i += kWarps * 32) {
+        const int r = i / n, c = i - r * n, a = row_adapter[r];
         float v = 0.0f;
-        if (has) {
+        if (first_part[r] < first_part[r + 1]) {
+            const float *hidden = sums + first_part[r] * p.rank;
+            const WT *up = static_cast<const WT *>(p.up) + static_cast<std::int64_t>(a) * p.rank * n + c;
 #pragma unroll 8
-            for (int k = 0; k < p.rank; ++k) v = fmaf(hidden[k], load1(up + k * p.n + c), v);
-            v *= factor;
+            for (int k = 0; k < p.rank; ++k) v = fmaf(hidden[k], load1(up + static_cast<std::int64_t>(k) * n), v);
+            v *= p.alpha * (p.scale != nullptr ? __ldg(p.scale + a) : 1.0f);
         }
-        float *out = p.out + row * p.out_ld + c;
+        float *out = p.out + (row0 + r) * p.out_ld + c;
         if (p.beta != 0.0f) v = fmaf(p.beta, *out, v);
-        *out = p.epilogue == CB200_EPILOGUE_NONE ? v : apply_epilogue(v, epilogue_has_bias(p.epilogue) ? __ldg(p.bias + c) : 0.0f, p.epilogue);
+        *out = finish_output(v, p.bias, c, p.epilogue);
     }
 }
 
 template<int BITS, typename WT, int V>
-cb200_status launch(adapter_params p, std::int64_t rows, int warps, cudaStream_t stream) {
+cb200_status launch(adapter_params p, std::int64_t rows, cudaStream_t stream) {
     p.lanes = 1;
     while (p.lanes < 32 && p.lanes * V < p.rank) p.lanes *= 2;
-    const std::size_t smem = static_cast<std::size_t>(kMostParts) * p.rank * sizeof(float);
-    qcsr_adapter_kernel<BITS, WT, V><<<static_cast<unsigned>(rows), warps * 32, smem, stream>>>(p);
+    const std::size_t smem = static_cast<std::size_t>(p.block_rows) * kMostParts * p.rank * sizeof(float);
+    qcsr_adapter_kernel<BITS, WT, V><<<static_cast<unsigned>((rows + p.block_rows - 1) / p.block_rows), kWarps * 32, smem, stream>>>(p);
     count_launch();
     CB200_CUDA_OK(cudaGetLastError());
     return CB200_STATUS_SUCCESS;
@@ -184,12 +253,12 @@ cb200_status launch(adapter_params p, std::int64_t rows, int warps, cudaStream_t
 
 // Elements of a lane's slice of A: 16 bytes where every row starts on such a boundary, else 8, else one element.
 template<int BITS, typename WT>
-cb200_status dispatch(const adapter_params &p, std::int64_t rows, int warps, cudaStream_t stream) {
+cb200_status dispatch(const adapter_params &p, std::int64_t rows, cudaStream_t stream) {
     constexpr int widest = 16 / static_cast<int>(sizeof(WT));
     const std::uintptr_t base = reinterpret_cast<std::uintptr_t>(p.down);
-    if (p.rank % widest == 0 && base % 16u == 0u) return launch<BITS, WT, widest>(p, rows, warps, stream);
-    if (p.rank % (widest / 2) == 0 && base % 8u == 0u) return launch<BITS, WT, widest / 2>(p, rows, warps, stream);
-    return launch<BITS, WT, 1>(p, rows, warps, stream);
+    if (p.rank % widest == 0 && base % 16u == 0u) return launch<BITS, WT, widest>(p, rows, stream);
+    if (p.rank % (widest / 2) == 0 && base % 8u == 0u) return launch<BITS, WT, widest / 2>(p, rows, stream);
+    return launch<BITS, WT, 1>(p, rows, stream);
 }
 
 } // namespace
@@ -212,8 +281,8 @@ extern "C" cb200_status cb200_qcsr_adapters(const cb200_adapters *d, void *strea
         return fail(CB200_STATUS_UNSUPPORTED, "unknown epilogue kind %d", d->epilogue);
     const bool bias_kind = d->epilogue == CB200_EPILOGUE_BIAS || d->epilogue >= CB200_EPILOGUE_BIAS_RELU;
     if (d->rank < 1 || d->rank > kMostRank) return fail(CB200_STATUS_UNSUPPORTED, "rank %lld outside 1 .. %d", (long long)d->rank, kMostRank);
-    if (d->n < 0 || d->adapters < 0 || x->rows < 0 || x->cols < 0 || x->cols > 0x7fffffffll || x->nnz < 0 || d->n > 0x7fffffffll || d->adapters > 0x7fffffffll)
-        return fail(CB200_STATUS_INVALID_SHAPE, "a size is negative or above 2^31");
+    if (d->n < 0 || d->adapters < 0 || x->rows < 0 || x->cols < 0 || x->cols > 0x7fffffffll || x->nnz < 0 || d->n > (1ll << 27) || d->adapters > 0x7fffffffll)
+        return fail(CB200_STATUS_INVALID_SHAPE, "a size is negative or too large (n up to 2^27, the others below 2^31)");
     if (d->out_ld < d->n) return fail(CB200_STATUS_INVALID_SHAPE, "leading dimension smaller than n");
     const std::int64_t begin = d->row_begin, end = d->row_end == CB200_ALL_ROWS ? x->rows : d->row_end;
     if (begin < 0 || end > x->rows || begin > end)
@@ -241,10 +310,16 @@ extern "C" cb200_status cb200_qcsr_adapters(const cb200_adapters *d, void *strea
     p.row_begin = begin; p.cols = x->cols; p.adapters = d->adapters; p.out_ld = d->out_ld; p.n = d->n;
     p.alpha = d->alpha; p.beta = d->beta;
     p.rank = static_cast<int>(d->rank); p.policy = x->policy; p.epilogue = d->epilogue;
-    const std::int64_t mean = x->nnz / std::max<std::int64_t>(x->rows, 1);
-    const int warps = static_cast<int>(std::min<std::int64_t>(kMostWarps, std::max<std::int64_t>(2, (mean + kSegment - 1) / kSegment)));
+    p.row_end = end;
+    // Rows of a block: about 8,192 entries, so that blocks are long enough to hide their start and end, but blocks enough for every SM,
+    // and no more parts than the shared memory holds.
+    const double mean = static_cast<double>(x->nnz) / static_cast<double>(std::max<std::int64_t>(x->rows, 1));
+    p.block_rows = 1;
+    while (2 * p.block_rows <= kMostRows && 2 * p.block_rows * mean <= 8192.0 && end - begin >= 4ll * 148 * p.block_rows &&
+           2 * p.block_rows * kMostParts * p.rank * static_cast<int>(sizeof(float)) <= kSumsBytes)
+        p.block_rows *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf16 = d->weight_dtype == CB200_DTYPE_BF16;
-    if (x->bits == 8) return bf16 ? dispatch<8, __nv_bfloat16>(p, end - begin, warps, s) : dispatch<8, float>(p, end - begin, warps, s);
-    return bf16 ? dispatch<4, __nv_bfloat16>(p, end - begin, warps, s) : dispatch<4, float>(p, end - begin, warps, s);
+    if (x->bits == 8) return bf16 ? dispatch<8, __nv_bfloat16>(p, end - begin, s) : dispatch<8, float>(p, end - begin, s);
+    return bf16 ? dispatch<4, __nv_bfloat16>(p, end - begin, s) : dispatch<4, float>(p, end - begin, s);
 }

@@ -46,7 +46,8 @@ inline bool rows_compatible(const row_matrix &out, const row_matrix &in, std::in
     return apart >= in_width && apart + out_width <= in.pitch;
 }
 
-// Columns that one load or store takes: 4, 2 or 1, by the alignment of every row.
+// Columns that one load or store takes: 4, 2 or 1, so that every row is whole accesses, each of them aligned.
+inline int columns_of_access(std::int64_t columns) { return columns % 4 == 0 ? 4 : columns % 2 == 0 ? 2 : 1; }
 inline int columns_per_access(const row_matrix &m, int most) {
     const int bytes = element_bytes(m.dtype);
     while (most > 1 && (reinterpret_cast<std::uintptr_t>(m.base) % static_cast<unsigned>(most * bytes) != 0u || m.pitch % (most * bytes) != 0)) most /= 2;
@@ -59,57 +60,38 @@ template<int SIZE>
 struct raw_quad {
     std::uint32_t w[SIZE];
 
-    // columns col ... col + 3 of the row at `row`; those from n on are zero
-    __device__ __forceinline__ void load(const unsigned char *row, int col, int n, int per_access) {
-        const unsigned char *p = row + static_cast<std::int64_t>(col) * SIZE;
-        if (col + 4 <= n) {
-            if (per_access == 4) {
-                if constexpr (SIZE == 4) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    w[0] = v.x; w[1] = v.y;
-                }
-            } else if (per_access == 2) {
-                if constexpr (SIZE == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p), u = *reinterpret_cast<const uint2 *>(p + 8);
-                    w[0] = v.x; w[1] = v.y; w[2] = u.x; w[3] = u.y;
-                } else {
-                    w[0] = *reinterpret_cast<const std::uint32_t *>(p);
-                    w[1] = *reinterpret_cast<const std::uint32_t *>(p + 4);
-                }
-            } else {
-                if constexpr (SIZE == 4) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = reinterpret_cast<const std::uint32_t *>(p)[k];
-                } else {
-                    const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
-                    const std::uint32_t h0 = h[0], h1 = h[1], h2 = h[2], h3 = h[3];
-                    w[0] = h0 | h1 << 16;
-                    w[1] = h2 | h3 << 16;
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < SIZE; ++k) w[k] = 0u;
-        if (col < n) {
-            if constexpr (SIZE == 4) {
-#pragma unroll
-                for (int k = 0; k < 3; ++k)
-                    if (col + k < n) w[k] = reinterpret_cast<const std::uint32_t *>(p)[k];
-            } else {
-                const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
-                w[0] = h[0];
-                if (col + 1 < n) w[0] |= static_cast<std::uint32_t>(h[1]) << 16;
-                if (col + 2 < n) w[1] = h[2];
-            }
-        }
-    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int k = 0; k < SIZE; ++k) w[k] = 0u;
+    }
+    // those of its columns at p that are among the `count` left of the row, in loads of PER_ACCESS elements; the others are zero
+    template<int PER_ACCESS>
+    __device__ __forceinline__ void load(const unsigned char *p, int count) {
+        clear();
+        if constexpr (SIZE == 4 && PER_ACCESS == 4) {
+            if (count <= 0) return;
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if constexpr (SIZE * PER_ACCESS == 8) {
+#pragma unroll
+            for (int k = 0; k < SIZE; k += 2) {
+                if (k * 4 / SIZE >= count) continue;
+                const uint2 v = *reinterpret_cast<const uint2 *>(p + 4 * k);
+                w[k] = v.x;
+                w[k + 1] = v.y;
+            }
+        } else if constexpr (SIZE * PER_ACCESS == 4) {
+#pragma unroll
+            for (int k = 0; k < SIZE; ++k)
+                if (k * 4 / SIZE < count) w[k] = *reinterpret_cast<const std::uint32_t *>(p + 4 * k);
+        } else {
+            std::uint32_t h[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < count) h[k] = reinterpret_cast<const unsigned short *>(p)[k];
+            w[0] = h[0] | h[1] << 16;
+            w[1] = h[2] | h[3] << 16;
+        }
     }
     // half: fp16 and not bf16, of two-byte elements
     __device__ __forceinline__ void widen(bool half, float (&v)[4]) const {
@@ -132,6 +114,20 @@ struct raw_quad {
     }
 };
 
+template<int PER_ACCESS, int SIZE, int Q>
+__device__ __forceinline__ void load_quads_by(const unsigned char *row, const int (&col)[Q], int n, raw_quad<SIZE> (&raw)[Q]) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) raw[i].template load<PER_ACCESS>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i]);
+}
+// Quads of a row of n columns, starting at columns col[i]; columns from n on are zero.  Nothing waits for a load here, but for
+// two-byte elements one by one, which are put together.
+template<int SIZE, int Q>
+__device__ __forceinline__ void load_quads(const unsigned char *row, const int (&col)[Q], int n, int per_access, raw_quad<SIZE> (&raw)[Q]) {
+    if (per_access == 4) load_quads_by<4>(row, col, n, raw);
+    else if (per_access == 2) load_quads_by<2>(row, col, n, raw);
+    else load_quads_by<1>(row, col, n, raw);
+}
+
 __device__ __forceinline__ std::uint32_t pack_pair(float lo, float hi, bool half) {
     std::uint32_t w;
     if (half) {
@@ -144,36 +140,66 @@ __device__ __forceinline__ std::uint32_t pack_pair(float lo, float hi, bool half
     return w;
 }
 
-// One rounding, to nearest, where the type has fewer bits than fp32.
-__device__ __forceinline__ void store_quad(unsigned char *row, int col, int n, int per_access, int dtype, const float (&v)[4]) {
-    if (col >= n) return;
-    if (dtype == CB200_DTYPE_F32) {
-        float *p = reinterpret_cast<float *>(row) + col;
-        if (col + 4 <= n && per_access == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else if (col + 4 <= n && per_access == 2) {
-            reinterpret_cast<float2 *>(p)[0] = make_float2(v[0], v[1]);
-            reinterpret_cast<float2 *>(p)[1] = make_float2(v[2], v[3]);
-        } else {
+// A quad's elements of SIZE bytes, packed: those among the `count` left of the row.
+template<int PER_ACCESS, int SIZE>
+__device__ __forceinline__ void store_quad(unsigned char *p, int count, const std::uint32_t (&w)[SIZE]) {
+    if constexpr (SIZE == 4 && PER_ACCESS == 4) {
+        if (count > 0) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (SIZE * PER_ACCESS == 8) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (col + k < n) p[k] = v[k];
-        }
-        return;
-    }
-    const bool half = dtype == CB200_DTYPE_F16;
-    unsigned short *p = reinterpret_cast<unsigned short *>(row) + col;
-    const std::uint32_t lo = pack_pair(v[0], v[1], half), hi = pack_pair(v[2], v[3], half);
-    if (col + 4 <= n && per_access == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
-    else if (col + 4 <= n && per_access == 2) {
-        reinterpret_cast<std::uint32_t *>(p)[0] = lo;
-        reinterpret_cast<std::uint32_t *>(p)[1] = hi;
+        for (int k = 0; k < SIZE; k += 2)
+            if (k * 4 / SIZE < count) *reinterpret_cast<uint2 *>(p + 4 * k) = make_uint2(w[k], w[k + 1]);
+    } else if constexpr (SIZE * PER_ACCESS == 4) {
+#pragma unroll
+        for (int k = 0; k < SIZE; ++k)
+            if (k * 4 / SIZE < count) *reinterpret_cast<std::uint32_t *>(p + 4 * k) = w[k];
     } else {
-        const unsigned short e[4] = {static_cast<unsigned short>(lo), static_cast<unsigned short>(lo >> 16), static_cast<unsigned short>(hi),
-                                     static_cast<unsigned short>(hi >> 16)};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (col + k < n) p[k] = e[k];
+            if (k < count) reinterpret_cast<unsigned short *>(p)[k] = static_cast<unsigned short>(w[k / 2] >> (16 * (k & 1)));
     }
+}
+template<int SIZE, int Q>
+__device__ __forceinline__ void store_packed(unsigned char *row, const int (&col)[Q], int n, int per_access, const std::uint32_t (&w)[Q][SIZE]) {
+    if (per_access == 4) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) store_quad<4>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+    } else if (per_access == 2) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) store_quad<2>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) store_quad<1>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+    }
+}
+// Values of quads into a row of n columns.  One rounding, to nearest, where the type has fewer bits than fp32.
+template<int Q>
+__device__ __forceinline__ void store_quads(unsigned char *row, const int (&col)[Q], int n, int per_access, int dtype, const float (&v)[Q][4]) {
+    if (dtype == CB200_DTYPE_F32) {
+        std::uint32_t w[Q][4];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[i][k] = __float_as_uint(v[i][k]);
+        }
+        store_packed<4>(row, col, n, per_access, w);
+        return;
+    }
+    std::uint32_t w[Q][2];
+    if (dtype == CB200_DTYPE_F16) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            w[i][0] = pack_pair(v[i][0], v[i][1], true);
+            w[i][1] = pack_pair(v[i][2], v[i][3], true);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            w[i][0] = pack_pair(v[i][0], v[i][1], false);
+            w[i][1] = pack_pair(v[i][2], v[i][3], false);
+        }
+    }
+    store_packed<2>(row, col, n, per_access, w);
 }
 #endif
 
