@@ -468,59 +468,58 @@ assert _DROPOUT_MATRIX.size == C.sizeof(capi.DropoutMatrix)
 assert _LAYER_NORM.size == C.sizeof(capi.LayerNorm)
 assert _ADAPTERS.size == C.sizeof(capi.Adapters)
 _packed_entries: dict = {}
+_F32 = torch.float32
 
 
-def _call_packed(name: str, structure: bytes, device) -> None:
-    """An entry point that takes one structure, as bytes, and the device's current stream."""
+def _call_packed(name: str, structure: bytes, index: int) -> None:
+    """An entry point that takes one structure, as bytes, and the current stream of device `index`."""
     entry = _packed_entries.get(name)
     if entry is None:
         entry = _packed_entries[name] = C.CFUNCTYPE(C.c_int32, C.c_char_p, C.c_void_p)((name, capi.lib()))
-    status = entry(structure, _stream_handle(device))
+    status = entry(structure, torch._C._cuda_getCurrentRawStream(index))
     if status:
         capi.check(status)
 
 
-def _index(device) -> int:
-    return torch.cuda.current_device() if device.index is None else device.index
-
-
-def _rows_of(t: torch.Tensor, name: str, shape=None) -> int:
-    """The type code of a matrix of rows that a row operator takes, which is checked."""
-    code = _TORCH_ROWS.get(t.dtype)
+def _rows_of(t: torch.Tensor, name: str, shape=None):
+    """(type code, shape, leading dimension) of a matrix of rows that a row operator takes, which is checked."""
+    code, size, stride = _TORCH_ROWS.get(t.dtype), t.shape, t.stride()
     if code is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16")
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    if len(size) != 2 or (stride[1] != 1 and size[1] > 1):
         raise ValueError(f"{name} must be a matrix whose rows are contiguous")
-    if shape is not None and t.shape != shape:
+    if shape is not None and size != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}")
-    return code
+    return code, size, stride[0]
 
 
-def _vector(t: torch.Tensor | None, name: str, length: int, dtype=torch.float32) -> int:
+def _vector(t: torch.Tensor | None, name: str, length: int, dtype=_F32) -> int:
     """Address of an optional vector, which is checked; 0 for None."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != length or (t.stride(0) != 1 and length > 1):
+    if t.dtype is not dtype or t.shape != (length,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} vector of {length}")
     return t.data_ptr()
 
 
-def _together(device, *tensors) -> None:
-    """The operands of a call live on one CUDA device."""
-    if device.type != "cuda":
+def _together(index: int, *tensors) -> None:
+    """The operands of a call live on CUDA device `index`."""
+    if index < 0:
         raise ValueError("the operands must be on a CUDA device")
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"operands on {t.device} and {device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"operands on {t.device} and cuda:{index}")
 
 
 def _generator(probability: float, seed: int, sequence: int, first_row: int, device_sequence):
     """The fields of a cb200_dropout."""
     if not 0 <= seed < 1 << 64 or not 0 <= sequence < 1 << 64:
         raise ValueError("seed and sequence are whole numbers below 2^64")
-    if device_sequence is not None and (device_sequence.dtype not in (torch.int64, torch.uint64) or device_sequence.numel() != 1):
+    if device_sequence is None:
+        return probability, seed, sequence, 0, first_row
+    if device_sequence.dtype not in (torch.int64, torch.uint64) or device_sequence.numel() != 1:
         raise ValueError("device_sequence must be one 64-bit whole number")
-    return probability, seed, sequence, 0 if device_sequence is None else device_sequence.data_ptr(), first_row
+    return probability, seed, sequence, device_sequence.data_ptr(), first_row
 
 
 def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *, first_row: int = 0,
@@ -530,21 +529,35 @@ def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *
     The mask follows from probability, seed, sequence (a number for each use), row and column alone: the gradient is the same
     call on the gradient, and a shard passes the number of its first row.  device_sequence: one int64 on the device that is
     added to sequence when the kernel runs.  out may be x."""
-    code = _rows_of(x, "x")
+    code, shape, ld = _rows_of(x, "x")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out_code = _rows_of(out, "out", x.shape)
+        out = torch.empty_like(x)
+    out_code, _, out_ld = _rows_of(out, "out", shape)
     generator = _generator(probability, seed, sequence, first_row, device_sequence)
-    device = x.device
-    _together(device, out, device_sequence)
+    index = x.get_device()
+    _together(index, out, device_sequence)
     _call_packed("cb200_dropout_rows", _DROPOUT_MATRIX.pack(
-        capi.ABI_VERSION, _DROPOUT_MATRIX.size, x.shape[0], x.shape[1], x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), code,
-        out_code, *generator, _index(device)), device)
+        capi.ABI_VERSION, _DROPOUT_MATRIX.size, *shape, x.data_ptr(), ld, out.data_ptr(), out_ld, code, out_code, *generator, index), index)
     return out
 
 
-def _norm_epilogue(epilogue) -> int:
+def _epilogue_of(epilogue) -> int:
     return capi.EPILOGUE[epilogue] if isinstance(epilogue, str) else int(epilogue)
+
+
+def _rows_like(x: torch.Tensor, given: torch.Tensor | None, dtype: torch.dtype | None, name: str) -> torch.Tensor:
+    """The matrix of a result: the given one, or a new one of x's shape."""
+    if given is None:
+        return torch.empty_like(x) if dtype is None or dtype is x.dtype else torch.empty_like(x, dtype=dtype)
+    if dtype is not None and given.dtype is not dtype:
+        raise ValueError(f"{name} has another type than {name}_dtype")
+    return given
+
+
+def _stats_of(stats: torch.Tensor, rows: int) -> int:
+    if stats.dtype is not _F32 or stats.shape != (rows, 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be a contiguous float32 tensor of shape ({rows}, 2)")
+    return stats.data_ptr()
 
 
 def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5, *,
@@ -556,28 +569,19 @@ def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.T
     epilogue: "none", "relu", "gelu_erf" or "gelu_tanh".  The result has x's type, out_dtype or that of out (which may be x).
     stats, a float32 [rows, 2] tensor, receives each row's {mean, 1 / sqrt(var + eps)}, which layer_norm_backward reads.
     dropout is a probability; seed, sequence, first_row and device_sequence are those of ops.dropout."""
-    code = _rows_of(x, "x")
-    rows, columns = x.shape
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError("out has another type than out_dtype")
-    out_code = _rows_of(out, "out", x.shape)
+    code, shape, ld = _rows_of(x, "x")
+    rows, columns = shape
+    out = _rows_like(x, out, out_dtype, "out")
+    out_code, _, out_ld = _rows_of(out, "out", shape)
     gamma_ptr, beta_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns)
     stats_ptr = 0 if stats is None else _stats_of(stats, rows)
     generator = _generator(dropout, seed, sequence, first_row, device_sequence)
-    device = x.device
-    _together(device, gamma, beta, out, stats, device_sequence)
+    index = x.get_device()
+    _together(index, gamma, beta, out, stats, device_sequence)
     _call_packed("cb200_layer_norm_forward", _LAYER_NORM.pack(
-        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), x.stride(0), gamma_ptr, beta_ptr, code, _norm_epilogue(epilogue), eps,
-        _index(device), *generator, stats_ptr, out.data_ptr(), out.stride(0), 0, 0, 0, 0, out_code, 0, 0, 0, 0, 0, 0), device)
+        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), ld, gamma_ptr, beta_ptr, code, _epilogue_of(epilogue), eps, index,
+        *generator, stats_ptr, out.data_ptr(), out_ld, 0, 0, 0, 0, out_code, 0, 0, 0, 0, 0, 0), index)
     return out
-
-
-def _stats_of(stats: torch.Tensor, rows: int) -> int:
-    if stats.dtype != torch.float32 or stats.shape != (rows, 2) or not stats.is_contiguous():
-        raise ValueError(f"stats must be a contiguous float32 tensor of shape ({rows}, 2)")
-    return stats.data_ptr()
 
 
 def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, gamma: torch.Tensor | None = None,
@@ -590,37 +594,38 @@ def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, 
     dx has x's type, dx_dtype or that of dx (which may be x or dy); spmm_transpose takes it as fp32.  dgamma and dbeta are
     float32, None where gamma or beta is None.  workspace: a tensor of layer_norm_backward_workspace bytes, else taken from
     torch's allocator."""
-    code, dy_code = _rows_of(x, "x"), _rows_of(dy, "dy", x.shape)
-    rows, columns = x.shape
-    if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype if dx_dtype is None else dx_dtype, device=x.device)
-    elif dx_dtype is not None and dx.dtype != dx_dtype:
-        raise ValueError("dx has another type than dx_dtype")
-    dx_code = _rows_of(dx, "dx", x.shape)
-    gamma_ptr, beta_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns)
+    code, shape, ld = _rows_of(x, "x")
+    rows, columns = shape
+    dy_code, _, dy_ld = _rows_of(dy, "dy", shape)
+    dx = _rows_like(x, dx, dx_dtype, "dx")
+    dx_code, _, dx_ld = _rows_of(dx, "dx", shape)
+    gamma_ptr, beta_ptr, stats_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns), _stats_of(stats, rows)
     if dgamma is None and gamma is not None:
-        dgamma = torch.empty(columns, dtype=torch.float32, device=x.device)
+        dgamma = torch.empty_like(gamma)
     if dbeta is None and beta is not None:
-        dbeta = torch.empty(columns, dtype=torch.float32, device=x.device)
-    stats_ptr = _stats_of(stats, rows)
+        dbeta = torch.empty_like(beta)
     dgamma_ptr, dbeta_ptr = _vector(dgamma, "dgamma", columns), _vector(dbeta, "dbeta", columns)
-    if workspace is None and (dgamma_ptr or dbeta_ptr):
-        workspace = torch.empty(layer_norm_backward_workspace(rows, columns), dtype=torch.uint8, device=x.device)
+    workspace_ptr = workspace_bytes = 0
+    if workspace is None and (dgamma_ptr or dbeta_ptr) and rows:
+        workspace = stats.new_empty(layer_norm_backward_workspace(rows, columns) // 4)
+    if workspace is not None:
+        workspace_ptr, workspace_bytes = workspace.data_ptr(), workspace.nbytes
     generator = _generator(dropout, seed, sequence, first_row, device_sequence)
-    device = x.device
-    _together(device, dy, stats, gamma, beta, dx, dgamma, dbeta, workspace, device_sequence)
+    index = x.get_device()
+    _together(index, dy, stats, gamma, beta, dx, dgamma, dbeta, workspace, device_sequence)
     _call_packed("cb200_layer_norm_backward", _LAYER_NORM.pack(
-        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), x.stride(0), gamma_ptr, beta_ptr, code, _norm_epilogue(epilogue), 0.0,
-        _index(device), *generator, stats_ptr, 0, 0, dy.data_ptr(), dy.stride(0), dx.data_ptr(), dx.stride(0), 0, dy_code, dx_code,
-        dgamma_ptr, dbeta_ptr, 0 if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size()), device)
+        capi.ABI_VERSION, _LAYER_NORM.size, rows, columns, x.data_ptr(), ld, gamma_ptr, beta_ptr, code, _epilogue_of(epilogue), 0.0, index,
+        *generator, stats_ptr, 0, 0, dy.data_ptr(), dy_ld, dx.data_ptr(), dx_ld, 0, dy_code, dx_code, dgamma_ptr, dbeta_ptr, workspace_ptr,
+        workspace_bytes), index)
     return dx, dgamma, dbeta
 
 
 def layer_norm_backward_workspace(rows: int, columns: int) -> int:
     """Bytes that layer_norm_backward needs for the sums of dgamma and dbeta."""
     need = C.c_uint64()
-    capi.check(capi.lib().cb200_layer_norm_backward_workspace(rows, columns, C.byref(need)))
+    status = capi.lib().cb200_layer_norm_backward_workspace(rows, columns, C.byref(need))
+    if status:
+        capi.check(status)
     return need.value
 
 
@@ -642,18 +647,18 @@ def adapter_forward(x: QuantizedCsr, adapter: torch.Tensor, down: torch.Tensor, 
         raise ValueError("down and up must be contiguous")
     adapter_ptr = _vector(adapter, "adapter", x.rows, torch.int32)
     scale_ptr, bias_ptr = _vector(scale, "scale", adapters), _vector(bias, "bias", n)
-    device = x.device
+    index = down.get_device()
     if out is None:
         if beta != 0.0:
             raise ValueError("beta needs an out to add to")
-        out = torch.empty(x.rows, n, dtype=torch.float32, device=device)
-    if out.dtype != torch.float32 or out.shape != (x.rows, n) or (out.stride(1) != 1 and n > 1):
+        out = torch.empty((x.rows, n), dtype=_F32, device=down.device)
+    stride = out.stride()
+    if out.dtype is not _F32 or out.shape != (x.rows, n) or (stride[1] != 1 and n > 1):
         raise ValueError(f"out must be a float32 matrix of shape ({x.rows}, {n}) whose rows are contiguous")
-    _together(device, adapter, down, up, scale, out, bias)
+    _together(index, x.row_ptr, adapter, up, scale, out, bias)
     _call_packed("cb200_qcsr_adapters", _ADAPTERS.pack(
         capi.ABI_VERSION, _ADAPTERS.size, x._bound()[2], adapter_ptr, adapters, rank, n, down.data_ptr(), up.data_ptr(), scale_ptr,
-        _TORCH_DENSE[down.dtype], _norm_epilogue(epilogue), out.data_ptr(), out.stride(0), alpha, beta, bias_ptr, row_begin, row_end,
-        _index(device)), device)
+        _TORCH_DENSE[down.dtype], _epilogue_of(epilogue), out.data_ptr(), stride[0], alpha, beta, bias_ptr, row_begin, row_end, index), index)
     return out
 
 
