@@ -4,11 +4,12 @@
 #include "row_quads.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cb200 {
 namespace {
 
-constexpr int kThreads = 256, kInFlight = 4;
+constexpr int kThreads = 256, kInFlight = 4, kBlocks = 3; // resident on an SM
 
 struct dropout_params {
     row_matrix x, y;
@@ -22,8 +23,8 @@ struct dropout_params {
 // A thread works on pieces of Q quads that lie a launch's width apart; it goes from one to the next by adding rows and pieces,
 // with no division.  Q = 2 for two-byte elements in rows of whole 16-byte pieces, where a piece is one load and one store.
 // WHOLE: rows are whole pieces and every access is aligned.
-template<int SIZE, int Q, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const dropout_params p) {
+template<int SIZE, bool HALVES, int Q, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, kBlocks) dropout_kernel(const dropout_params p) {
     const std::uint64_t first = static_cast<std::uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
     const std::uint64_t sequence = sequence_of(p.drop);
     const bool half = p.x.dtype == CB200_DTYPE_F16;
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const dropout_params 
                 raw[i][0].template load<4>(x + static_cast<std::uint64_t>(at[i]) * (4u * SIZE), 4);
             } else {
                 const int col[1] = {static_cast<int>(at[i]) * 4};
-                load_quads<SIZE, 1>(x, col, p.columns, p.per_access, raw[i]);
+                load_quads(x, col, p.columns, p.per_access, raw[i]);
             }
         }
 #pragma unroll
@@ -62,33 +63,33 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const dropout_params 
             float v[Q][4];
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                raw[i][q].widen(half, v[q]);
+                raw[i][q].template widen<HALVES>(half, v[q]);
                 if (p.drop.on) drop_quad(p.drop, sequence, r[i], at[i] * Q + q, v[q]);
             }
             unsigned char *y = p.y.base + r[i] * p.y.pitch;
             if constexpr (WHOLE && Q == 2) { // a result of two bytes as well
-                const bool y_half = p.y.dtype == CB200_DTYPE_F16;
+                const bool y_half = HALVES && p.y.dtype == CB200_DTYPE_F16;
                 *reinterpret_cast<uint4 *>(y + static_cast<std::uint64_t>(at[i]) * 16u) =
                     make_uint4(pack_pair(v[0][0], v[0][1], y_half), pack_pair(v[0][2], v[0][3], y_half), pack_pair(v[1][0], v[1][1], y_half),
                                pack_pair(v[1][2], v[1][3], y_half));
             } else {
                 const int col[1] = {static_cast<int>(at[i]) * 4};
-                store_quads<1>(y, col, p.columns, WHOLE ? 4 : p.per_access, p.y.dtype, v);
+                store_quads<HALVES>(y, col, p.columns, WHOLE ? 4 : p.per_access, p.y.dtype, v);
             }
         }
     }
 }
 
-template<int SIZE, int Q, bool WHOLE>
+template<int SIZE, bool HALVES, int Q, bool WHOLE>
 cb200_status launch(dropout_params p, std::int64_t rows, cudaStream_t stream) {
     p.rows = static_cast<std::uint32_t>(rows);
     p.pieces = static_cast<std::uint32_t>((p.columns + 4ll * Q - 1) / (4 * Q));
     const std::int64_t threads = (rows * static_cast<std::int64_t>(p.pieces) + kInFlight - 1) / kInFlight;
-    const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>((threads + kThreads - 1) / kThreads, 148 * 8));
+    const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>((threads + kThreads - 1) / kThreads, 148 * kBlocks));
     const std::int64_t step = static_cast<std::int64_t>(grid) * kThreads;
     p.step_rows = static_cast<std::uint32_t>(step / p.pieces);
     p.step_pieces = static_cast<std::uint32_t>(step % p.pieces);
-    dropout_kernel<SIZE, Q, WHOLE><<<grid, kThreads, 0, stream>>>(p);
+    dropout_kernel<SIZE, HALVES, Q, WHOLE><<<grid, kThreads, 0, stream>>>(p);
     count_launch();
     CB200_CUDA_OK(cudaGetLastError());
     return CB200_STATUS_SUCCESS;
@@ -117,8 +118,12 @@ extern "C" cb200_status cb200_dropout_rows(const cb200_dropout_matrix *m, void *
     p.per_access = columns_per_access(p.y, columns_per_access(p.x, columns_of_access(m->columns)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool whole = p.per_access == 4;
-    if (element_bytes(p.x.dtype) == 4) return whole ? launch<4, 1, true>(p, m->rows, s) : launch<4, 1, false>(p, m->rows, s);
-    if (whole && element_bytes(p.y.dtype) == 2 && p.columns % 8 == 0 && columns_per_access(p.x, 8) == 8 && columns_per_access(p.y, 8) == 8)
-        return launch<2, 2, true>(p, m->rows, s);
-    return whole ? launch<2, 1, true>(p, m->rows, s) : launch<2, 1, false>(p, m->rows, s);
+    const auto run = [&](auto halves) {
+        constexpr bool H = decltype(halves)::value;
+        if (element_bytes(p.x.dtype) == 4) return whole ? launch<4, H, 1, true>(p, m->rows, s) : launch<4, H, 1, false>(p, m->rows, s);
+        if (whole && element_bytes(p.y.dtype) == 2 && p.columns % 8 == 0 && columns_per_access(p.x, 8) == 8 && columns_per_access(p.y, 8) == 8)
+            return launch<2, H, 2, true>(p, m->rows, s);
+        return whole ? launch<2, H, 1, true>(p, m->rows, s) : launch<2, H, 1, false>(p, m->rows, s);
+    };
+    return p.x.dtype == CB200_DTYPE_F16 || p.y.dtype == CB200_DTYPE_F16 ? run(std::true_type{}) : run(std::false_type{});
 }

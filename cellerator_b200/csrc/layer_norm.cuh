@@ -17,10 +17,9 @@ constexpr int kNarrowColumns = 512;
 constexpr std::int64_t kMostColumns = 65536;
 constexpr int kNarrowThreads = 256;
 constexpr int kNarrowItems = 4; // quads of a row that a lane holds
-// Most threads of a block of a wide row, by the quads of a thread.  Three quads and twelve warps: three warps to a scheduler leave
-// each thread 168 registers, and eight such blocks hold 36,864 columns.
-constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 3 ? 384 : 512; }
-constexpr int kMostWarps = 16;
+// Most threads of a block of a wide row, by the quads of a thread: eight blocks hold 36,864 columns with two, all 65,536 with four.
+constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 2 ? 576 : 512; }
+constexpr int kMostWarps = 18;
 constexpr int kMostCluster = 8;
 
 struct layer_norm_params {
@@ -43,12 +42,12 @@ struct layer_norm_params {
 struct wide_shape {
     int quads_per_thread, cluster, threads, slice_quads;
 };
-// As few blocks to a row as hold it (the sums of a row that one block holds need no cluster barrier), with three quads to a thread
+// As few blocks to a row as hold it (the sums of a row that one block holds need no cluster barrier), with two quads to a thread
 // where eight blocks suffice.
 inline wide_shape wide_shape_of(std::int64_t columns) {
     wide_shape s{};
     const int quads = static_cast<int>((columns + 3) / 4);
-    s.quads_per_thread = quads <= 3 * wide_threads(3) * kMostCluster ? 3 : 4;
+    s.quads_per_thread = quads <= 2 * wide_threads(2) * kMostCluster ? 2 : 4;
     s.cluster = 1;
     while (s.cluster < kMostCluster && quads > s.quads_per_thread * wide_threads(s.quads_per_thread) * s.cluster) s.cluster *= 2;
     s.slice_quads = (quads + s.cluster - 1) / s.cluster;
@@ -58,7 +57,7 @@ inline wide_shape wide_shape_of(std::int64_t columns) {
 
 // Launches a kernel of a wide row as clusters.
 template<typename K>
-cudaError_t launch_wide(K kernel, const layer_norm_params &p, const wide_shape &shape, unsigned clusters, cudaStream_t stream) {
+cudaError_t launch_wide(K kernel, const layer_norm_params &p, const wide_shape &shape, unsigned clusters, std::size_t smem, cudaStream_t stream) {
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = static_cast<unsigned>(shape.cluster);
@@ -66,16 +65,17 @@ cudaError_t launch_wide(K kernel, const layer_norm_params &p, const wide_shape &
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(clusters * static_cast<unsigned>(shape.cluster));
     config.blockDim = dim3(static_cast<unsigned>(shape.threads));
+    config.dynamicSmemBytes = smem;
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = shape.cluster > 1 ? 1u : 0u;
     return cudaLaunchKernelEx(&config, kernel, p);
 }
 
-// Clusters of this shape that the device holds at once, at least one.  Asked for once for each shape (the answer is a
-// property of the kernel and the device).
+// Clusters of this shape that the device holds at once, at least one.  Asked for once for each shape, whose shared memory follows
+// from it (the answer is a property of the kernel and the device).
 template<auto kernel>
-unsigned resident_clusters(const wide_shape &shape, int device) {
+unsigned resident_clusters(const wide_shape &shape, std::size_t smem, int device) {
     constexpr int kDevices = 64;
     static std::atomic<unsigned> known[kDevices][kMostCluster + 1][kMostWarps + 1];
     const bool kept = device >= 0 && device < kDevices;
@@ -92,12 +92,13 @@ unsigned resident_clusters(const wide_shape &shape, int device) {
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(static_cast<unsigned>(shape.cluster));
         config.blockDim = dim3(static_cast<unsigned>(shape.threads));
+        config.dynamicSmemBytes = smem;
         config.attrs = &attribute;
         config.numAttrs = 1;
         if (cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess) found = 0;
     } else {
         int per_sm = 0, sms = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, shape.threads, 0) == cudaSuccess &&
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, shape.threads, smem) == cudaSuccess &&
             cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess)
             found = per_sm * sms;
     }
@@ -200,6 +201,40 @@ __device__ __forceinline__ float through_activation(float dy, float z) {
         return dy * (steep > 0.0f ? fmaf(z * steep, 1.5957691216057308f * fmaf(0.134145f, zz, 1.0f), gate) : gate);
     }
     return dy;
+}
+
+// Some quads at once: the choices are made once for all of them, as a branch for each costs a quarter of the instructions.
+template<int KIND, int Q>
+__device__ __forceinline__ void activate_as(float (&v)[Q][4]) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(v[i][k]);
+    }
+}
+template<int Q>
+__device__ __forceinline__ void activate(int kind, float (&v)[Q][4]) {
+    if (kind == CB200_EPILOGUE_NONE) return;
+    if (kind == CB200_EPILOGUE_RELU) activate_as<CB200_EPILOGUE_RELU>(v);
+    else if (kind == CB200_EPILOGUE_GELU_ERF) activate_as<CB200_EPILOGUE_GELU_ERF>(v);
+    else activate_as<CB200_EPILOGUE_GELU_TANH>(v);
+}
+// dz in place of dy, from u
+template<int KIND, int Q>
+__device__ __forceinline__ void through_as(float (&dy)[Q][4], const float (&u)[Q][4], const float4 (&gamma)[Q], const float4 (&beta)[Q]) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        dy[i][0] = through_activation<KIND>(dy[i][0], fmaf(u[i][0], gamma[i].x, beta[i].x));
+        dy[i][1] = through_activation<KIND>(dy[i][1], fmaf(u[i][1], gamma[i].y, beta[i].y));
+        dy[i][2] = through_activation<KIND>(dy[i][2], fmaf(u[i][2], gamma[i].z, beta[i].z));
+        dy[i][3] = through_activation<KIND>(dy[i][3], fmaf(u[i][3], gamma[i].w, beta[i].w));
+    }
+}
+template<int Q>
+__device__ __forceinline__ void drop_quads(const dropout_args &d, std::uint64_t sequence, std::uint32_t row, const int (&col)[Q], float (&v)[Q][4]) {
+    if (!d.on) return;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) drop_quad(d, sequence, row, static_cast<std::uint32_t>(col[i]) >> 2, v[i]);
 }
 
 // Sums over groups of `lanes` neighbouring lanes (a power of two), in each of them.

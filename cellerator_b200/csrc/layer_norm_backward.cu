@@ -16,36 +16,49 @@ constexpr int kNarrowBlocks = 3; // narrow: resident on an SM, with two quads a 
 constexpr int kNarrowParts = 148 * kNarrowBlocks;
 constexpr int kWideParts = 148 * 4;
 
-// dz and u of a quad in place of dy and x; h u added to sums[1], h to sums[0]
-template<int KIND>
-struct quad_terms {
-    float mean, rstd;
-
-    __device__ __forceinline__ void apply(float (&x)[4], float (&dy)[4], const float (&gamma)[4], const float (&beta)[4], float (&dgamma)[4],
-                                          float (&dbeta)[4], float (&sums)[2]) const {
+// u and h in place of x and dy of some quads of a row; dz u and dz added to what the thread keeps of their columns, h and h u to the
+// row's sums.  at: where the quads' gamma (and, beta_at further, beta) stand in shared memory.
+template<int KIND, int Q>
+__device__ __forceinline__ void row_terms(float mean, float rstd, const float *gamma_at, int beta_at, const int (&at)[Q], float (&x)[Q][4], float (&dy)[Q][4],
+                                          float (&dgamma)[Q][4], float (&dbeta)[Q][4], float (&sums)[2]) {
+    float4 gamma[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        gamma[i] = *reinterpret_cast<const float4 *>(gamma_at + at[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] = (x[i][k] - mean) * rstd;
+    }
+    if constexpr (KIND != CB200_EPILOGUE_NONE) {
+        float4 beta[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) beta[i] = *reinterpret_cast<const float4 *>(gamma_at + beta_at + at[i]);
+        through_as<KIND>(dy, x, gamma, beta);
+    }
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        const float g[4] = {gamma[i].x, gamma[i].y, gamma[i].z, gamma[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            x[k] = (x[k] - mean) * rstd;
-            dy[k] = through_activation<KIND>(dy[k], fmaf(x[k], gamma[k], beta[k]));
-            dbeta[k] += dy[k];
-            dgamma[k] = fmaf(dy[k], x[k], dgamma[k]);
-            dy[k] *= gamma[k];
-            sums[0] += dy[k];
-            sums[1] = fmaf(dy[k], x[k], sums[1]);
+            dbeta[i][k] += dy[i][k];
+            dgamma[i][k] = fmaf(dy[i][k], x[i][k], dgamma[i][k]);
+            dy[i][k] *= g[k];
+            sums[0] += dy[i][k];
+            sums[1] = fmaf(dy[i][k], x[i][k], sums[1]);
         }
     }
-};
+}
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  Columns past the last hold
 // zeros in dy, so that they add nothing.
-template<int SX, int SG, int KIND, int ITEMS>
+template<int SX, int SG, bool HALVES, int KIND, int ITEMS>
 __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : kNarrowBlocks - 1) layer_norm_back_narrow_kernel(const layer_norm_params p) {
     __shared__ float meet[kNarrowThreads / 32][ITEMS * 4 * 32];
-    __shared__ __align__(16) float parameters[2][ITEMS * 4 * 32]; // gamma and beta: registers are short here
+    constexpr int kParameters = ITEMS * 4 * 32 + 4;
+    __shared__ __align__(16) float parameters[2][kParameters]; // gamma and beta: registers are short here
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
     const bool half = p.x.dtype == CB200_DTYPE_F16, half_dy = p.dy.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    for (int c = threadIdx.x; c < ITEMS * 4 * 32; c += kNarrowThreads) {
+    for (int c = threadIdx.x; c < kParameters; c += kNarrowThreads) {
         parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
         parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
     }
@@ -54,7 +67,7 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
     int col[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        col[i] = min((i * p.lanes + in_row) * 4, p.columns);
+        col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
 #pragma unroll
         for (int k = 0; k < 4; ++k) dgamma[i][k] = dbeta[i][k] = 0.0f;
     }
@@ -73,22 +86,17 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
     fetch(row);
     for (; row - group < p.rows; row += step) {
         const bool active = row < p.rows;
-        const quad_terms<KIND> terms{stats.x, stats.y};
+        const float mean = stats.x, rstd = stats.y;
         float x[ITEMS][4], dy[ITEMS][4], sums[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            raw_x[i].widen(half, x[i]);
-            raw_dy[i].widen(half_dy, dy[i]);
+            raw_x[i].template widen<HALVES>(half, x[i]);
+            raw_dy[i].template widen<HALVES>(half_dy, dy[i]);
         }
         fetch(row + step);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            if (!active || col[i] >= p.columns) continue;
-            if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), dy[i]);
-            float gamma[4], beta[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            *reinterpret_cast<float4 *>(gamma) = *reinterpret_cast<const float4 *>(parameters[0] + col[i]);
-            if constexpr (KIND != CB200_EPILOGUE_NONE) *reinterpret_cast<float4 *>(beta) = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
-            terms.apply(x[i], dy[i], gamma, beta, dgamma[i], dbeta[i], sums);
+        if (active) {
+            drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, dy);
+            row_terms<KIND>(mean, rstd, parameters[0], kParameters, col, x, dy, dgamma, dbeta, sums);
         }
         lane_sums(sums, p.lanes);
         sums[0] *= inverse;
@@ -97,9 +105,9 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][k] = terms.rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
+            for (int k = 0; k < 4; ++k) x[i][k] = rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
         }
-        store_quads(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, x);
+        store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, x);
     }
     let_next_launch_start();
     if (p.partials == nullptr) return;
@@ -112,7 +120,7 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
             for (int k = 0; k < 4; ++k) {
                 float v = which == 0 ? dgamma[i][k] : dbeta[i][k];
                 for (int off = p.lanes; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-                if (group == 0) meet[warp][(i * p.lanes + in_row) * 4 + k] = v;
+                if (group == 0) meet[warp][(i * p.lanes + in_row) * 4 + k] = v; // columns past the row's end hold nothing that is read
             }
         }
         __syncthreads();
@@ -128,52 +136,58 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
 }
 
 // A block, or a cluster of blocks that take a slice of the columns each, per row; a thread keeps the sums of its columns from row
-// to row.  In a cluster the two sums of a row go round while the row before is written and the one behind is worked on.
-template<int SX, int SG, int KIND, int QT, bool CLUSTER>
+// to row.  In a cluster the two sums of a row go round while the row before is written and the one behind is worked on.  gamma and
+// beta of the slice are in shared memory: the sums, two rows and the next one's values take the registers.
+template<int SX, int SG, bool HALVES, int QT, bool CLUSTER>
 __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(const layer_norm_params p) {
     __shared__ wide_notes<2, CLUSTER> notes;
-    const int lane = threadIdx.x & 31, all_warps = p.cluster * (blockDim.x >> 5);
+    extern __shared__ __align__(16) float parameters[]; // gamma and beta of the block's quads, and a quad each for threads without
+    const int lane = threadIdx.x & 31, all_warps = p.cluster * (blockDim.x >> 5), n = p.columns;
     const int rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
     const std::int64_t first = CLUSTER ? blockIdx.x / p.cluster : blockIdx.x, stride = CLUSTER ? gridDim.x / p.cluster : gridDim.x;
     const bool half = p.x.dtype == CB200_DTYPE_F16, half_dy = p.dy.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    float gamma[QT][4], beta[QT][4], dgamma[QT][4], dbeta[QT][4];
-    int col[QT];
+    const int beta_at = (p.slice_quads + 1) * 4, column0 = rank * p.slice_quads * 4;
+    for (int c = threadIdx.x; c < beta_at; c += blockDim.x) {
+        const bool in = column0 + c < n && c < p.slice_quads * 4;
+        parameters[c] = p.gamma != nullptr && in ? __ldg(p.gamma + column0 + c) : 1.0f;
+        parameters[beta_at + c] = p.beta != nullptr && in ? __ldg(p.beta + column0 + c) : 0.0f;
+    }
+    float dgamma[QT][4], dbeta[QT][4];
+    int col[QT], at[QT];
     wide_columns<QT>(p, rank, col);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
-        load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
+        at[i] = min(i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x), p.slice_quads) * 4;
 #pragma unroll
         for (int k = 0; k < 4; ++k) dgamma[i][k] = dbeta[i][k] = 0.0f;
     }
-    const float inverse = 1.0f / static_cast<float>(p.columns);
+    const float inverse = 1.0f / static_cast<float>(n);
     raw_quad<SX> raw_x[QT];
     raw_quad<SG> raw_dy[QT];
     float2 stats;
-    const auto fetch = [&](std::int64_t at) {
-        if (at >= p.rows) return;
-        stats = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
-        load_quads(p.x.base + at * p.x.pitch, col, p.columns, p.per_access, raw_x);
-        load_quads(p.dy.base + at * p.dy.pitch, col, p.columns, p.per_access, raw_dy);
+    const auto fetch = [&](std::int64_t row) {
+        if (row >= p.rows) return;
+        stats = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
+        load_quads(p.x.base + row * p.x.pitch, col, n, p.per_access, raw_x);
+        load_quads(p.dy.base + row * p.dy.pitch, col, n, p.per_access, raw_dy);
     };
     float x[QT][4], dy[QT][4]; // x and dy of a row, then its u and h
     const auto widened = [&]() {
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-            raw_x[i].widen(half, x[i]);
-            raw_dy[i].widen(half_dy, dy[i]);
+            raw_x[i].template widen<HALVES>(half, x[i]);
+            raw_dy[i].template widen<HALVES>(half_dy, dy[i]);
         }
     };
     const auto summed = [&](std::int64_t row, float2 of_row, float (&sums)[2]) {
-        const quad_terms<KIND> terms{of_row.x, of_row.y};
         sums[0] = sums[1] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            if (col[i] >= p.columns) continue;
-            if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), dy[i]);
-            terms.apply(x[i], dy[i], gamma[i], beta[i], dgamma[i], dbeta[i], sums);
-        }
+        drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, dy);
+        const auto terms = [&](auto kind) { row_terms<decltype(kind)::value>(of_row.x, of_row.y, parameters, beta_at, at, x, dy, dgamma, dbeta, sums); };
+        if (p.epilogue == CB200_EPILOGUE_NONE) terms(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
+        else if (p.epilogue == CB200_EPILOGUE_RELU) terms(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
+        else if (p.epilogue == CB200_EPILOGUE_GELU_ERF) terms(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
+        else terms(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
         warp_sums<2>(sums);
     };
     const auto finish = [&](const float (&u)[QT][4], const float (&h)[QT][4], std::int64_t row, float rstd, int set) {
@@ -192,9 +206,10 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[i][k] = rstd * (h[i][k] - sums[0] - u[i][k] * sums[1]);
         }
-        store_quads(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, v);
+        store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, n, p.per_access, p.dx.dtype, v);
     };
     fetch(first);
+    __syncthreads();
     int set = 0;
     float sums[2];
     if constexpr (CLUSTER) {
@@ -236,14 +251,14 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(
     }
     let_next_launch_start();
     if (p.partials == nullptr) return;
-    float *out = p.partials + first * 2 * p.columns;
+    float *out = p.partials + first * 2 * n;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (col[i] + k >= p.columns) continue;
+            if (col[i] + k >= n) continue;
             out[col[i] + k] = dgamma[i][k];
-            out[p.columns + col[i] + k] = dbeta[i][k];
+            out[n + col[i] + k] = dbeta[i][k];
         }
     }
 }
@@ -292,25 +307,27 @@ struct backward_launch {
     }
     template<auto kernel>
     cb200_status wide(const wide_shape &shape) const {
-        const std::int64_t parts = std::min<std::int64_t>({p.rows, kWideParts / shape.cluster, resident_clusters<kernel>(shape, device)});
-        CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(parts), stream));
+        const std::size_t smem = static_cast<std::size_t>(shape.slice_quads + 1) * 32u; // up to 37 KB with two quads to a thread, 66 KB with four
+        if (shape.quads_per_thread != 2) CB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 66 * 1024));
+        const std::int64_t parts = std::min<std::int64_t>({p.rows, kWideParts / shape.cluster, resident_clusters<kernel>(shape, smem, device)});
+        CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(parts), smem, stream));
         return finish(parts);
     }
-    template<int SX, int SG, int KIND>
+    template<int SX, int SG, bool HALVES, int KIND>
     cb200_status run() {
         if (p.columns <= kNarrowColumns) {
             const std::int64_t parts = narrow_parts(p.rows, p.columns);
             p.lanes = narrow_lanes(p.columns, back_items(p.columns));
-            if (back_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
-            else layer_norm_back_narrow_kernel<SX, SG, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            if (back_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, HALVES, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            else layer_norm_back_narrow_kernel<SX, SG, HALVES, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             return finish(parts);
         }
         const wide_shape shape = wide_shape_of(p.columns);
         p.cluster = shape.cluster;
         p.slice_quads = shape.slice_quads;
-        if (shape.cluster == 1) return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 3, false>>(shape);
-        if (shape.quads_per_thread == 3) return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 3, true>>(shape);
-        return wide<layer_norm_back_wide_kernel<SX, SG, KIND, 4, true>>(shape);
+        if (shape.cluster == 1) return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 2, false>>(shape);
+        if (shape.quads_per_thread == 2) return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 2, true>>(shape);
+        return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 4, true>>(shape);
     }
 };
 
@@ -369,7 +386,12 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
     if (!sums && p.dx.base == nullptr) return CB200_STATUS_SUCCESS;
     const bool wide_x = element_bytes(p.x.dtype) == 4, wide_dy = element_bytes(p.dy.dtype) == 4;
     return with_epilogue(p.epilogue, [&](auto kind) {
-        if (wide_x) return wide_dy ? b.run<4, 4, kind()>() : b.run<4, 2, kind()>();
-        return wide_dy ? b.run<2, 4, kind()>() : b.run<2, 2, kind()>();
+        const auto of_sizes = [&](auto halves) {
+            constexpr bool H = decltype(halves)::value;
+            if (wide_x) return wide_dy ? b.run<4, 4, H, kind()>() : b.run<4, 2, H, kind()>();
+            return wide_dy ? b.run<2, 4, H, kind()>() : b.run<2, 2, H, kind()>();
+        };
+        return p.x.dtype == CB200_DTYPE_F16 || p.dy.dtype == CB200_DTYPE_F16 || (p.dx.base != nullptr && p.dx.dtype == CB200_DTYPE_F16) ? of_sizes(std::true_type{})
+                                                                                                                                        : of_sizes(std::false_type{});
     });
 }

@@ -11,32 +11,30 @@ constexpr int kNarrowBlocks = 3; // resident on an SM
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
 // shared memory: a lane's sixteen columns of them would take a third of its registers.
-template<int SIZE, int KIND>
+template<int SIZE, bool HALVES, int KIND>
 __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narrow_kernel(const layer_norm_params p) {
-    __shared__ __align__(16) float parameters[2][kNarrowColumns];
+    __shared__ __align__(16) float parameters[2][kNarrowColumns + 4];
     const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
-    const bool half = p.x.dtype == CB200_DTYPE_F16, affine = p.gamma != nullptr || p.beta != nullptr;
+    const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
     int col[kNarrowItems];
 #pragma unroll
-    for (int i = 0; i < kNarrowItems; ++i) col[i] = min((i * p.lanes + in_row) * 4, p.columns);
+    for (int i = 0; i < kNarrowItems; ++i) col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
     const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
     std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
     raw_quad<SIZE> raw[kNarrowItems];
     if (row < p.rows) load_quads(p.x.base + row * p.x.pitch, col, p.columns, p.per_access, raw);
-    if (affine) {
-        for (int c = threadIdx.x; c < kNarrowColumns; c += kNarrowThreads) {
-            parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
-            parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
-        }
-        __syncthreads();
+    for (int c = threadIdx.x; c < kNarrowColumns + 4; c += kNarrowThreads) {
+        parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
+        parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
     }
+    __syncthreads();
     for (; row - group < p.rows; row += step) {
         float v[kNarrowItems][4], sum[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < kNarrowItems; ++i) {
-            raw[i].widen(half, v[i]);
+            raw[i].template widen<HALVES>(half, v[i]);
             sum[0] += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
         }
         if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
@@ -60,34 +58,179 @@ __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narr
         if (row >= p.rows) continue;
         if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
-            if (col[i] >= p.columns) continue;
-            if (affine) {
-                const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
-                v[i][0] = activation<KIND>(fmaf(v[i][0] * rstd, g.x, b.x));
-                v[i][1] = activation<KIND>(fmaf(v[i][1] * rstd, g.y, b.y));
-                v[i][2] = activation<KIND>(fmaf(v[i][2] * rstd, g.z, b.z));
-                v[i][3] = activation<KIND>(fmaf(v[i][3] * rstd, g.w, b.w));
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(v[i][k] * rstd);
-            }
-            if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
+        for (int i = 0; i < kNarrowItems; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
+            const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
+            v[i][0] = fmaf(v[i][0] * rstd, g.x, b.x);
+            v[i][1] = fmaf(v[i][1] * rstd, g.y, b.y);
+            v[i][2] = fmaf(v[i][2] * rstd, g.z, b.z);
+            v[i][3] = fmaf(v[i][3] * rstd, g.w, b.w);
         }
-        store_quads(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
+        activate_as<KIND>(v);
+        drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
+        store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
     }
+}
+
+// A block per row, the row in registers, its next row on the way where two fit; gamma and beta stay in shared memory from row to
+// row, as many columns of them as it holds (the rest of beta comes out of L2).  Each warp takes the mean of its columns and the
+// squares of what differs from that; from all warps' numbers come the row's mean and variance,
+//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
+// with one barrier between them.
+constexpr int kRowThreads = 1024;
+constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
+constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
+
+// The quads of a thread lie a block's width apart; only the last of them can reach past the row's end.
+template<int SIZE, bool HALVES, int QT>
+__global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const layer_norm_params p, int beta_quads) {
+    constexpr bool kAhead = QT * SIZE <= 16; // registers for two rows
+    extern __shared__ __align__(16) float parameters[]; // gamma, then beta of each thread's first beta_quads quads
+    __shared__ float notes[2][2][32], sizes[32], inverses[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = p.columns, width = static_cast<int>(blockDim.x) * 4;
+    const bool half = p.x.dtype == CB200_DTYPE_F16;
+    const std::uint64_t sequence = sequence_of(p.drop);
+    const int padded = (n + 3) & ~3;
+    const float *beta_at = parameters + padded + 4; // behind each there is room for a quad past the row's end
+    const bool beta_vectors = p.beta != nullptr && reinterpret_cast<std::uintptr_t>(p.beta) % 16u == 0u;
+    int col[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i) col[i] = i * width + static_cast<int>(threadIdx.x) * 4;
+    col[QT - 1] = min(col[QT - 1], padded);
+    std::int64_t row = blockIdx.x;
+    raw_quad<SIZE> now[QT], next[kAhead ? QT : 1];
+    load_quads<QT - 1>(p.x.base + row * p.x.pitch, col, n, p.per_access, now);
+    for (int c = threadIdx.x; c < padded + 4; c += blockDim.x) {
+        parameters[c] = p.gamma != nullptr && c < n ? __ldg(p.gamma + c) : 1.0f;
+        if (c < beta_quads * width) parameters[padded + 4 + c] = p.beta != nullptr && c < n ? __ldg(p.beta + c) : 0.0f;
+    }
+    const int left = n - (QT - 1) * width - warp * 128; // columns of the warp's last quads
+    const float size = static_cast<float>((QT - 1) * 128 + min(max(left, 0), 128)), inverse_size = 1.0f / size, count = static_cast<float>(n), inverse = 1.0f / count;
+    if (lane == 0) {
+        sizes[warp] = size;
+        inverses[warp] = inverse_size;
+    }
+    const float own_columns = static_cast<float>(4 * (QT - 1) + min(max(n - col[QT - 1], 0), 4)), own_inverse = 1.0f / own_columns;
+    int set = 0;
+    for (; row < p.rows; row += gridDim.x, set ^= 1) {
+        if constexpr (kAhead) {
+            if (row + gridDim.x < p.rows) load_quads<QT - 1>(p.x.base + (row + gridDim.x) * p.x.pitch, col, n, p.per_access, next);
+        }
+        // this thread's columns about the mean of its first quad, in one walk: the square of how far that is from the mean of all of
+        // them is at most (QT - 1) times their variance, so no digits are lost to the difference at the end
+        float centre, moved, spread;
+        {
+            float v[4];
+            now[0].template widen<HALVES>(half, v);
+            centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
+            const pair minus(-centre);
+            pair s(0.0f), q(0.0f);
+#pragma unroll
+            for (int i = 0; i < QT; ++i) {
+                now[i].template widen<HALVES>(half, v);
+                if (i == QT - 1 && col[i] + 4 > n) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (col[i] + k >= n) v[k] = centre;
+                }
+                const pair d = pair(v[0], v[1]) + minus, e = pair(v[2], v[3]) + minus;
+                s = s + d;
+                q = fma(d, d, q);
+                s = s + e;
+                q = fma(e, e, q);
+            }
+            moved = s.sum();
+            spread = q.sum();
+        }
+        // {sum, sum of squares about the warp's mean} of the warp
+        float t[1] = {fmaf(own_columns, centre, moved)};
+        const float own_off = moved * own_inverse; // of the thread's mean from its centre
+        warp_sums(t);
+        if (lane == 0) notes[set][0][warp] = t[0];
+        {
+            const float differs = (centre - t[0] * inverse_size) + own_off;
+            t[0] = fmaf(own_columns * differs, differs, fmaf(-moved, own_off, spread));
+        }
+        warp_sums(t);
+        if (lane == 0) notes[set][1][warp] = t[0];
+        __syncthreads();
+        const float of_warp = lane < warps ? notes[set][0][lane] : 0.0f;
+        t[0] = of_warp;
+        warp_sums(t);
+        const float mean = t[0] / count; // exact for rows of one value
+        t[0] = 0.0f;
+        if (lane < warps) {
+            const float differs = fmaf(of_warp, inverses[lane], -mean);
+            t[0] = fmaf(sizes[lane] * differs, differs, notes[set][1][lane]);
+        }
+        warp_sums(t);
+        const float rstd = rsqrtf(fmaf(t[0], inverse, p.epsilon));
+        if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+        // a few quads at a time: what is computed takes twice the registers of what was loaded
+        constexpr int B = QT % 3 == 0 ? 3 : 2;
+        unsigned char *y = p.y.base + row * p.y.pitch;
+#pragma unroll
+        for (int first = 0; first < QT; first += B) {
+            float v[B][4];
+            int at[B];
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const int i = first + j;
+                at[j] = col[i];
+                now[i].template widen<HALVES>(half, v[j]);
+                const float4 g = *reinterpret_cast<const float4 *>(parameters + at[j]);
+                float b[4];
+                if (i < beta_quads) *reinterpret_cast<float4 *>(b) = *reinterpret_cast<const float4 *>(beta_at + at[j]);
+                else if (i < QT - 1 && beta_vectors) *reinterpret_cast<float4 *>(b) = __ldg(reinterpret_cast<const float4 *>(p.beta + at[j]));
+                else load_parameters(p.beta, at[j], n, 0.0f, b);
+                v[j][0] = fmaf((v[j][0] - mean) * rstd, g.x, b[0]);
+                v[j][1] = fmaf((v[j][1] - mean) * rstd, g.y, b[1]);
+                v[j][2] = fmaf((v[j][2] - mean) * rstd, g.z, b[2]);
+                v[j][3] = fmaf((v[j][3] - mean) * rstd, g.w, b[3]);
+            }
+            activate(p.epilogue, v);
+            drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), at, v);
+            if (first + B < QT) store_quads<HALVES, B>(y, at, n, p.per_access, p.y.dtype, v);
+            else store_quads<HALVES, B - 1>(y, at, n, p.per_access, p.y.dtype, v);
+        }
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int i = 0; i < QT; ++i) now[i] = next[i];
+        } else {
+            if (row + gridDim.x < p.rows) load_quads<QT - 1>(p.x.base + (row + gridDim.x) * p.x.pitch, col, n, p.per_access, now);
+        }
+    }
+}
+
+template<int SIZE, bool HALVES, int QT>
+cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t stream) {
+    constexpr auto kernel = layer_norm_row_kernel<SIZE, HALVES, QT>;
+    const int quads = (p.columns + 3) / 4, threads = ((quads + QT - 1) / QT + 31) / 32 * 32;
+    const std::size_t gamma_bytes = static_cast<std::size_t>(quads + 1) * 16u, width = static_cast<std::size_t>(threads) * 16u;
+    const std::size_t beta_quads = std::min<std::size_t>(QT, (kRowShared - gamma_bytes) / width), beta_bytes = beta_quads == QT ? gamma_bytes : beta_quads * width;
+    // more than the default 48 KB is asked for once per kernel and device
+    static std::atomic<bool> asked[64];
+    if (gamma_bytes + beta_bytes > 40 * 1024 && !(device < 64 && asked[device].load(std::memory_order_relaxed))) {
+        CB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRowShared)));
+        if (device < 64) asked[device].store(true, std::memory_order_relaxed);
+    }
+    const std::int64_t by_shared = kRowShared / (gamma_bytes + beta_bytes + 1024), resident = std::max<std::int64_t>(1, std::min<std::int64_t>({kRowThreads / threads, by_shared, 32}));
+    const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>(p.rows, 148 * resident));
+    kernel<<<grid, threads, gamma_bytes + beta_bytes, stream>>>(p, static_cast<int>(beta_quads));
+    count_launch();
+    CB200_CUDA_OK(cudaGetLastError());
+    return CB200_STATUS_SUCCESS;
 }
 
 // Rows of a step of a wide kernel.
 template<int SIZE, int QT>
-constexpr int kWideRows = (QT == 3 ? 8 : 4) / SIZE;
+constexpr int kWideRows = (QT == 2 ? 8 : 4) / SIZE;
 
 // A block, or a cluster of blocks that take a slice of the columns each, works on R rows at a time.  Each warp takes the mean of
 // its columns and the squares of what differs from that; from all warps' numbers come the row's mean and variance,
 //     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
 // with one exchange between them.  In a cluster the exchange of one step of rows goes round while the step before is written
 // and the one behind it is summed.
-template<int SIZE, int KIND, int QT, bool CLUSTER>
+template<int SIZE, bool HALVES, int QT, bool CLUSTER>
 __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const layer_norm_params p) {
     constexpr int R = kWideRows<SIZE, QT>;
     __shared__ wide_notes<2 * R, CLUSTER> notes;
@@ -136,7 +279,7 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
                 float x[4];
-                now[r][i].widen(half, x);
+                now[r][i].template widen<HALVES>(half, x);
                 t[r] += (x[0] + x[1]) + (x[2] + x[3]);
             }
         }
@@ -149,7 +292,7 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
                 float x[4];
-                now[r][i].widen(half, x);
+                now[r][i].template widen<HALVES>(half, x);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[k] -= mean;
                 if (col[i] + 4 > p.columns) {
@@ -194,12 +337,13 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
             float v[QT][4];
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
-                raw[r][i].widen(half, v[i]);
+                raw[r][i].template widen<HALVES>(half, v[i]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(fmaf((v[i][k] - mean[r]) * rstd, gamma[i][k], beta[i][k]));
-                if (p.drop.on) drop_quad(p.drop, sequence, static_cast<std::uint32_t>(row), static_cast<std::uint32_t>(col[i] >> 2), v[i]);
+                for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - mean[r]) * rstd, gamma[i][k], beta[i][k]);
             }
-            store_quads(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
+            activate(p.epilogue, v);
+            drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
+            store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
         }
     };
 
@@ -245,31 +389,34 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const
     }
 }
 
-template<int SIZE, int KIND, int QT, bool CLUSTER>
+template<int SIZE, bool HALVES, int QT, bool CLUSTER>
 cb200_status launch_wide_forward(const layer_norm_params &p, const wide_shape &shape, int device, cudaStream_t stream) {
-    constexpr auto kernel = layer_norm_wide_kernel<SIZE, KIND, QT, CLUSTER>;
+    constexpr auto kernel = layer_norm_wide_kernel<SIZE, HALVES, QT, CLUSTER>;
     constexpr int step = kWideRows<SIZE, QT>;
-    const std::int64_t clusters = std::min<std::int64_t>((p.rows + step - 1) / step, resident_clusters<kernel>(shape, device));
-    CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(clusters), stream));
+    const std::int64_t clusters = std::min<std::int64_t>((p.rows + step - 1) / step, resident_clusters<kernel>(shape, 0, device));
+    CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(clusters), 0, stream));
     count_launch();
     return CB200_STATUS_SUCCESS;
 }
 
-template<int SIZE, int KIND>
+template<int SIZE, bool HALVES, int KIND>
 cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream) {
     if (p.columns <= kNarrowColumns) {
         const std::int64_t per_block = kNarrowThreads / p.lanes, blocks = (p.rows + per_block - 1) / per_block;
-        layer_norm_narrow_kernel<SIZE, KIND><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
+        layer_norm_narrow_kernel<SIZE, HALVES, KIND><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
         count_launch();
         CB200_CUDA_OK(cudaGetLastError());
         return CB200_STATUS_SUCCESS;
     }
+    // quads of a thread: all but its last lie in the row, with blocks that are a multiple of 32 threads, from 64, 376, 937 and 2,520 quads on
+    if (p.columns <= 2048) return launch_rows<SIZE, HALVES, 2>(p, device, stream);
+    if (p.columns <= 4 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 4>(p, device, stream);
+    if (p.columns <= 6 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 6>(p, device, stream);
+    if (p.columns <= kRowColumns) return launch_rows<SIZE, HALVES, 9>(p, device, stream);
     const wide_shape shape = wide_shape_of(p.columns);
     p.cluster = shape.cluster;
     p.slice_quads = shape.slice_quads;
-    if (shape.cluster == 1) return launch_wide_forward<SIZE, KIND, 3, false>(p, shape, device, stream);
-    if (shape.quads_per_thread == 3) return launch_wide_forward<SIZE, KIND, 3, true>(p, shape, device, stream);
-    return launch_wide_forward<SIZE, KIND, 4, true>(p, shape, device, stream);
+    return launch_wide_forward<SIZE, HALVES, 4, true>(p, shape, device, stream);
 }
 
 } // namespace
@@ -289,6 +436,8 @@ extern "C" cb200_status cb200_layer_norm_forward(const cb200_layer_norm *d, void
     if (p.rows == 0) return CB200_STATUS_SUCCESS;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_epilogue(p.epilogue, [&](auto kind) {
-        return element_bytes(p.x.dtype) == 4 ? launch_forward<4, kind()>(p, d->device, s) : launch_forward<2, kind()>(p, d->device, s);
+        if (p.x.dtype == CB200_DTYPE_F16) return launch_forward<2, true, kind()>(p, d->device, s);
+        if (p.x.dtype == CB200_DTYPE_BF16) return p.y.dtype == CB200_DTYPE_F16 ? launch_forward<2, true, kind()>(p, d->device, s) : launch_forward<2, false, kind()>(p, d->device, s);
+        return p.y.dtype == CB200_DTYPE_F16 ? launch_forward<4, true, kind()>(p, d->device, s) : launch_forward<4, false, kind()>(p, d->device, s);
     });
 }

@@ -55,6 +55,31 @@ inline int columns_per_access(const row_matrix &m, int most) {
 }
 
 #if defined(__CUDACC__)
+// Two fp32 operations in one instruction: half the issue slots where a kernel is short of them.
+struct pair {
+    unsigned long long bits;
+    __device__ __forceinline__ pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ explicit pair(float both) : pair(both, both) {}
+    __device__ __forceinline__ void get(float &lo, float &hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(bits)); }
+    __device__ __forceinline__ float sum() const {
+        float lo, hi;
+        get(lo, hi);
+        return lo + hi;
+    }
+};
+__device__ __forceinline__ pair operator+(pair a, pair b) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.bits) : "l"(b.bits));
+    return a;
+}
+__device__ __forceinline__ pair operator*(pair a, pair b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.bits) : "l"(b.bits));
+    return a;
+}
+__device__ __forceinline__ pair fma(pair a, pair b, pair c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.bits) : "l"(a.bits), "l"(b.bits));
+    return c;
+}
+
 // The bits of a quad of elements of SIZE bytes.
 template<int SIZE>
 struct raw_quad {
@@ -93,12 +118,13 @@ struct raw_quad {
             w[1] = h[2] | h[3] << 16;
         }
     }
-    // half: fp16 and not bf16, of two-byte elements
+    // half: fp16 and not bf16, of two-byte elements.  HALVES: whether they can be at all; a choice at run time would convert both ways.
+    template<bool HALVES>
     __device__ __forceinline__ void widen(bool half, float (&v)[4]) const {
         if constexpr (SIZE == 4) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
-        } else if (half) {
+        } else if (HALVES && half) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 __half2 h;
@@ -114,18 +140,18 @@ struct raw_quad {
     }
 };
 
-template<int PER_ACCESS, int SIZE, int Q>
+template<int WHOLE, int PER_ACCESS, int SIZE, int Q>
 __device__ __forceinline__ void load_quads_by(const unsigned char *row, const int (&col)[Q], int n, raw_quad<SIZE> (&raw)[Q]) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) raw[i].template load<PER_ACCESS>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i]);
+    for (int i = 0; i < Q; ++i) raw[i].template load<PER_ACCESS>(row + static_cast<std::uint32_t>(col[i]) * SIZE, i < WHOLE ? 4 : n - col[i]);
 }
 // Quads of a row of n columns, starting at columns col[i]; columns from n on are zero.  Nothing waits for a load here, but for
-// two-byte elements one by one, which are put together.
-template<int SIZE, int Q>
+// two-byte elements one by one, which are put together.  WHOLE: so many of the quads, the first ones, are known to lie in the row.
+template<int WHOLE = 0, int SIZE, int Q>
 __device__ __forceinline__ void load_quads(const unsigned char *row, const int (&col)[Q], int n, int per_access, raw_quad<SIZE> (&raw)[Q]) {
-    if (per_access == 4) load_quads_by<4>(row, col, n, raw);
-    else if (per_access == 2) load_quads_by<2>(row, col, n, raw);
-    else load_quads_by<1>(row, col, n, raw);
+    if (per_access == 4) load_quads_by<WHOLE, 4>(row, col, n, raw);
+    else if (per_access == 2) load_quads_by<WHOLE, 2>(row, col, n, raw);
+    else load_quads_by<WHOLE, 1>(row, col, n, raw);
 }
 
 __device__ __forceinline__ std::uint32_t pack_pair(float lo, float hi, bool half) {
@@ -159,21 +185,22 @@ __device__ __forceinline__ void store_quad(unsigned char *p, int count, const st
             if (k < count) reinterpret_cast<unsigned short *>(p)[k] = static_cast<unsigned short>(w[k / 2] >> (16 * (k & 1)));
     }
 }
-template<int SIZE, int Q>
+template<int WHOLE, int SIZE, int Q>
 __device__ __forceinline__ void store_packed(unsigned char *row, const int (&col)[Q], int n, int per_access, const std::uint32_t (&w)[Q][SIZE]) {
     if (per_access == 4) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) store_quad<4>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+        for (int i = 0; i < Q; ++i) store_quad<4>(row + static_cast<std::uint32_t>(col[i]) * SIZE, i < WHOLE ? 4 : n - col[i], w[i]);
     } else if (per_access == 2) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) store_quad<2>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+        for (int i = 0; i < Q; ++i) store_quad<2>(row + static_cast<std::uint32_t>(col[i]) * SIZE, i < WHOLE ? 4 : n - col[i], w[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) store_quad<1>(row + static_cast<std::uint32_t>(col[i]) * SIZE, n - col[i], w[i]);
+        for (int i = 0; i < Q; ++i) store_quad<1>(row + static_cast<std::uint32_t>(col[i]) * SIZE, i < WHOLE ? 4 : n - col[i], w[i]);
     }
 }
-// Values of quads into a row of n columns.  One rounding, to nearest, where the type has fewer bits than fp32.
-template<int Q>
+// Values of quads into a row of n columns.  One rounding, to nearest, where the type has fewer bits than fp32.  HALVES as for widen,
+// WHOLE as for load_quads.
+template<bool HALVES, int WHOLE = 0, int Q>
 __device__ __forceinline__ void store_quads(unsigned char *row, const int (&col)[Q], int n, int per_access, int dtype, const float (&v)[Q][4]) {
     if (dtype == CB200_DTYPE_F32) {
         std::uint32_t w[Q][4];
@@ -182,24 +209,17 @@ __device__ __forceinline__ void store_quads(unsigned char *row, const int (&col)
 #pragma unroll
             for (int k = 0; k < 4; ++k) w[i][k] = __float_as_uint(v[i][k]);
         }
-        store_packed<4>(row, col, n, per_access, w);
+        store_packed<WHOLE>(row, col, n, per_access, w);
         return;
     }
+    const bool half = HALVES && dtype == CB200_DTYPE_F16;
     std::uint32_t w[Q][2];
-    if (dtype == CB200_DTYPE_F16) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            w[i][0] = pack_pair(v[i][0], v[i][1], true);
-            w[i][1] = pack_pair(v[i][2], v[i][3], true);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            w[i][0] = pack_pair(v[i][0], v[i][1], false);
-            w[i][1] = pack_pair(v[i][2], v[i][3], false);
-        }
+    for (int i = 0; i < Q; ++i) {
+        w[i][0] = pack_pair(v[i][0], v[i][1], half);
+        w[i][1] = pack_pair(v[i][2], v[i][3], half);
     }
-    store_packed<2>(row, col, n, per_access, w);
+    store_packed<WHOLE>(row, col, n, per_access, w);
 }
 #endif
 
