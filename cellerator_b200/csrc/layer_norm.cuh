@@ -237,6 +237,13 @@ __device__ __forceinline__ void drop_quads(const dropout_args &d, std::uint64_t 
     for (int i = 0; i < Q; ++i) drop_quad(d, sequence, row, static_cast<std::uint32_t>(col[i]) >> 2, v[i]);
 }
 
+// Brings `bytes` bytes at p on their way to L2, whole pieces of 16 bytes from the one that p lies in; p is not the start of its
+// allocation (a row behind the first), so that the bytes in front of it are there.
+__device__ __forceinline__ void prefetch_bytes(const unsigned char *p, std::uint32_t bytes) {
+    const std::uint64_t from = reinterpret_cast<std::uint64_t>(p) & ~std::uint64_t{15}, to = (reinterpret_cast<std::uint64_t>(p) + bytes) & ~std::uint64_t{15};
+    if (to > from) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(static_cast<std::uint32_t>(to - from)) : "memory");
+}
+
 // Sums over groups of `lanes` neighbouring lanes (a power of two), in each of them.
 template<int N>
 __device__ __forceinline__ void lane_sums(float (&v)[N], int lanes) {

@@ -162,12 +162,17 @@ __global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(
 #pragma unroll
         for (int k = 0; k < 4; ++k) dgamma[i][k] = dbeta[i][k] = 0.0f;
     }
+    const int own = min(p.slice_quads * 4, n - column0); // columns of the block
     const float inverse = 1.0f / static_cast<float>(n);
     raw_quad<SX> raw_x[QT];
     raw_quad<SG> raw_dy[QT];
     float2 stats;
     const auto fetch = [&](std::int64_t row) {
         if (row >= p.rows) return;
+        if (threadIdx.x == 0 && row + stride < p.rows && own > 0) { // the row behind it, on its way to L2
+            prefetch_bytes(p.x.base + (row + stride) * p.x.pitch + column0 * SX, static_cast<std::uint32_t>(own) * SX);
+            prefetch_bytes(p.dy.base + (row + stride) * p.dy.pitch + column0 * SG, static_cast<std::uint32_t>(own) * SG);
+        }
         stats = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
         load_quads(p.x.base + row * p.x.pitch, col, n, p.per_access, raw_x);
         load_quads(p.dy.base + row * p.dy.pitch, col, n, p.per_access, raw_dy);

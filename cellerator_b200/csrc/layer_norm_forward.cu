@@ -111,7 +111,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
     }
     const float own_columns = static_cast<float>(4 * (QT - 1) + min(max(n - col[QT - 1], 0), 4)), own_inverse = 1.0f / own_columns;
     int set = 0;
+    const std::int64_t ahead = kAhead ? 2 : 1; // rows, of this block's, that L2 is asked for in advance
     for (; row < p.rows; row += gridDim.x, set ^= 1) {
+        if (threadIdx.x == 0 && row + ahead * gridDim.x < p.rows)
+            prefetch_bytes(p.x.base + (row + ahead * gridDim.x) * p.x.pitch, static_cast<std::uint32_t>(n) * SIZE);
         if constexpr (kAhead) {
             if (row + gridDim.x < p.rows) load_quads<QT - 1>(p.x.base + (row + gridDim.x) * p.x.pitch, col, n, p.per_access, next);
         }
