@@ -38,9 +38,9 @@ struct adapter_params {
 };
 
 // Entries of a part of a row of `len` entries, a multiple of a warp's segment: by the length alone.
-__device__ __forceinline__ std::int64_t part_entries(std::int64_t len) {
-    const std::int64_t even = (len + kMostParts - 1) / kMostParts;
-    return max(static_cast<std::int64_t>(kSegment), (even + kSegment - 1) / kSegment * kSegment);
+__device__ __forceinline__ int part_entries(int len) {
+    const int even = (len + kMostParts - 1) / kMostParts;
+    return max(kSegment, (even + kSegment - 1) / kSegment * kSegment);
 }
 
 // V neighbouring elements of a row of A.
@@ -49,22 +49,21 @@ struct slice {
     static constexpr int bytes = V * static_cast<int>(sizeof(WT));
     static constexpr int words = bytes >= 4 ? bytes / 4 : 1;
     std::uint32_t w[words];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < words; ++i) w[i] = 0u;
-    }
     __device__ __forceinline__ void load(const unsigned char *p) {
-        if constexpr (bytes == 16) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        } else if constexpr (bytes == 8) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-            w[0] = v.x; w[1] = v.y;
-        } else if constexpr (bytes == 4) {
-            w[0] = __ldg(reinterpret_cast<const unsigned *>(p));
-        } else {
-            w[0] = __ldg(reinterpret_cast<const unsigned short *>(p));
+        // volatile: a batch of loads is issued before the first of its products
+        if constexpr (bytes == 16)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+        else if constexpr (bytes == 8) asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        else if constexpr (bytes == 4) asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+        else {
+            unsigned short h;
+            asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(h) : "l"(p));
+            w[0] = h;
         }
+    }
+    __device__ __forceinline__ void keep_if(bool held) {
+#pragma unroll
+        for (int i = 0; i < words; ++i) w[i] = held ? w[i] : 0u;
     }
     // acc += v * w; pairs of columns with the two-wide fp32 FMA
     __device__ __forceinline__ void add_to(float (&acc)[V], float v) const {
@@ -96,11 +95,13 @@ struct slice {
 // does not hold up the others.  A warp decodes 128 entries at a time into shared memory, {gene, value}, the next ones' indices and
 // codes being on their way meanwhile; then `lanes` lanes serve an entry, V columns of A each, 8 rows of A in flight.  A part's sum is
 // that of 32 / lanes classes of its entries, a row's that of its parts in order, and the product with B follows from shared memory.
+// Lanes past a part's end read its last entry again, and genes outside the matrix row 0 of A: both are staged as gene -1, whose row
+// counts as zeros whatever it holds.  Segments without such entries, nearly all, take the branch that does not look.
 template<int BITS, typename WT, int V>
 __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
     __shared__ __align__(16) int2 staged[kWarps][kSegment];
-    __shared__ std::int64_t row_start[kMostRows], code_start[kMostRows], row_len[kMostRows], row_share[kMostRows];
-    __shared__ int row_adapter[kMostRows], first_part[kMostRows + 1];
+    __shared__ std::int64_t row_start[kMostRows], code_start[kMostRows];
+    __shared__ int row_len[kMostRows], row_share[kMostRows], row_adapter[kMostRows], first_part[kMostRows + 1];
     extern __shared__ float sums[]; // [parts][rank]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const std::int64_t row0 = p.row_begin + static_cast<std::int64_t>(blockIdx.x) * p.block_rows;
@@ -109,14 +110,15 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
         int upto = 0;
         if (lane < rows) {
             const int a = __ldg(p.adapter + row0 + lane);
-            const bool has = a >= 0 && a < p.adapters;
-            const std::int64_t start = __ldg(p.row_ptr + row0 + lane), len = has ? __ldg(p.row_ptr + row0 + lane + 1) - start : 0, share = part_entries(len);
+            const bool has = a >= 0 && a < p.adapters && p.cols > 0;
+            const std::int64_t start = __ldg(p.row_ptr + row0 + lane);
+            const int len = has ? static_cast<int>(__ldg(p.row_ptr + row0 + lane + 1) - start) : 0, share = part_entries(len);
             row_adapter[lane] = has ? a : -1;
             row_start[lane] = start;
             row_len[lane] = len;
             row_share[lane] = share;
             code_start[lane] = p.packed_row_ptr != nullptr ? __ldg(p.packed_row_ptr + row0 + lane) : start;
-            upto = static_cast<int>((len + share - 1) / share);
+            upto = (len + share - 1) / share;
         }
 #pragma unroll
         for (int off = 1; off < kMostRows; off <<= 1) {
@@ -128,28 +130,27 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
     }
     __syncthreads();
     const int parts = first_part[rows];
-    const bool row_policy = p.policy == CB200_DECODE_COLUMN_SCALE_ROW_OFFSET;
+    const unsigned genes = static_cast<unsigned>(p.cols);
+    const bool row_policy = p.policy == CB200_DECODE_COLUMN_SCALE_ROW_OFFSET, by_gene = p.scales != nullptr && p.offsets != nullptr && !row_policy;
     const int lanes = p.lanes, groups = 32 / lanes, group = lane / lanes, in_row = lane & (lanes - 1);
     const unsigned row_bytes = static_cast<unsigned>(p.rank) * sizeof(WT);
     int2 *stage = staged[warp];
     for (int column0 = 0; column0 < p.rank; column0 += lanes * V) { // of A; one turn but for wide ranks of narrow slices
         const int col = column0 + in_row * V;
         const bool holds = col < p.rank;
-        int part = warp, r = 0, gene[kRuns];
+        int part = warp, r = 0, at = 0, to = 0; // entries of row r: those of the segment start at `at`
+        int gene[kRuns];
         unsigned code[kRuns];
-        std::int64_t at = 0, to = 0; // entries of row r: those of the segment start at `at`
         const auto fetch = [&]() {
-            const std::int32_t *cols = p.col_idx + row_start[r];
-            const std::uint8_t *codes = p.packed + code_start[r];
+            const std::int32_t *cols = p.col_idx + row_start[r] + at;
+            const std::uint8_t *codes = p.packed + code_start[r] + (BITS == 8 ? at : at >> 1); // `at` is even
+            const int last = to - at - 1;
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) {
-                const std::int64_t e = at + i * 32 + lane;
-                gene[i] = -1;
-                code[i] = 0u;
-                if (e >= to) continue;
-                gene[i] = __ldg(cols + e);
+                const int e = min(i * 32 + lane, last);
+                asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(gene[i]) : "l"(cols + e));
                 if constexpr (BITS == 8) code[i] = __ldg(codes + e);
-                else code[i] = (__ldg(codes + (e >> 1)) >> (4 * (e & 1))) & 15u;
+                else code[i] = __ldg(codes + (e >> 1)) >> (4 * (e & 1)) & 15u;
             }
         };
         const auto open = [&]() {
@@ -164,20 +165,37 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
         while (part < parts) {
-            const float row_offset = row_policy && p.offsets != nullptr ? __ldg(p.offsets + row0 + r) : 0.0f;
+            const int count = min(kSegment, to - at), part_now = part;
+            const unsigned char *down = p.down + static_cast<std::int64_t>(row_adapter[r]) * p.cols * row_bytes + (holds ? col : 0) * sizeof(WT);
+            float scale[kRuns], offset[kRuns];
+            bool fine = count == kSegment && holds;
+            unsigned at_gene[kRuns];
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) {
-                int2 entry = make_int2(-1, 0); // what is left out, and what lies behind the part's end
-                if (gene[i] >= 0 && gene[i] < p.cols) {
-                    const float scale = p.scales != nullptr ? __ldg(p.scales + gene[i]) : 1.0f;
-                    const float offset = row_policy ? row_offset : p.offsets != nullptr ? __ldg(p.offsets + gene[i]) : 0.0f;
-                    entry = make_int2(gene[i], __float_as_int(fmaf(static_cast<float>(code[i]), scale, offset)));
-                }
-                stage[i * 32 + lane] = entry;
+                const bool inside = static_cast<unsigned>(gene[i]) < genes;
+                fine = fine && inside;
+                at_gene[i] = inside ? static_cast<unsigned>(gene[i]) : 0u;
+                if (!inside || i * 32 + lane >= count) gene[i] = -1;
             }
+            if (by_gene) {
+#pragma unroll
+                for (int i = 0; i < kRuns; ++i) {
+                    scale[i] = __ldg(p.scales + at_gene[i]);
+                    offset[i] = __ldg(p.offsets + at_gene[i]);
+                }
+            } else {
+                const float row_offset = row_policy && p.offsets != nullptr ? __ldg(p.offsets + row0 + r) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < kRuns; ++i) {
+                    scale[i] = p.scales != nullptr ? __ldg(p.scales + at_gene[i]) : 1.0f;
+                    offset[i] = !row_policy && p.offsets != nullptr ? __ldg(p.offsets + at_gene[i]) : row_offset;
+                }
+            }
+            fine = __all_sync(0xffffffffu, fine);
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i)
+                stage[i * 32 + lane] = make_int2(gene[i], __float_as_int(fmaf(static_cast<float>(code[i]), scale[i], offset[i])));
             __syncwarp();
-            const unsigned char *down = p.down + static_cast<std::int64_t>(row_adapter[r]) * p.cols * row_bytes + col * sizeof(WT);
-            const int count = static_cast<int>(min(static_cast<std::int64_t>(kSegment), to - at)), part_now = part;
             at += kSegment;
             const bool ends = at >= to;
             if (ends) {
@@ -186,32 +204,52 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
             } else {
                 fetch();
             }
-            const auto add = [&](auto unrolled, int e) {
-                constexpr int U = decltype(unrolled)::value;
-                slice<WT, V> w[U];
-                float v[U];
+            const int2 *mine = stage + group;
+            if (fine) {
+                const auto add = [&](auto unrolled, int e) {
+                    constexpr int U = decltype(unrolled)::value;
+                    slice<WT, V> w[U];
+                    float v[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int2 entry = stage[e + u * groups];
-                    v[u] = __int_as_float(entry.y);
-                    w[u].clear();
-                    if (entry.x >= 0 && holds) w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(entry.x)) * row_bytes);
+                    for (int u = 0; u < U; ++u) {
+                        const int2 entry = mine[e + u * groups];
+                        v[u] = __int_as_float(entry.y);
+                        w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(entry.x)) * row_bytes);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) w[u].add_to(acc, v[u]);
+                };
+                if (groups == 32) add(std::integral_constant<int, 4>{}, 0); // one entry to a lane
+                else
+                    for (int e = 0; e < kSegment; e += 8 * groups) add(std::integral_constant<int, 8>{}, e);
+            } else {
+                for (int e = 0; e < count; e += 4 * groups) {
+                    slice<WT, V> w[4];
+                    float v[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int2 entry = mine[e + u * groups];
+                        const bool held = entry.x >= 0 && holds;
+                        v[u] = held ? __int_as_float(entry.y) : 0.0f;
+                        w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(max(entry.x, 0))) * row_bytes);
+                        w[u].keep_if(held);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) w[u].add_to(acc, v[u]);
                 }
-#pragma unroll
-                for (int u = 0; u < U; ++u) w[u].add_to(acc, v[u]);
-            };
-            // 128 / groups turns, 4 at least
-            int e = 0;
-            for (; e + 8 * groups <= kSegment && e < count; e += 8 * groups) add(std::integral_constant<int, 8>{}, e + group);
-            if (e < count) add(std::integral_constant<int, 4>{}, e + group); // 32 groups: one entry to a lane
+            }
             __syncwarp();
             if (!ends) continue;
+            for (int off = lanes; off < 32; off <<= 1) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                for (int off = lanes; off < 32; off <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
-                if (group == 0 && col + i < p.rank) sums[part_now * p.rank + col + i] = acc[i];
-                acc[i] = 0.0f;
+                for (int i = 0; i < V; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
             }
+            if (group == 0 && holds) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) sums[part_now * p.rank + col + i] = acc[i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = 0.0f;
         }
     }
     __syncthreads();
