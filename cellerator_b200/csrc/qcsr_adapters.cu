@@ -34,6 +34,7 @@ struct adapter_params {
     float alpha, beta;
     int rank, policy, epilogue;
     int lanes;      // that serve an entry: a power of two
+    int up_quads;   // B in columns of four
     int block_rows; // rows of a block
 };
 
@@ -90,6 +91,19 @@ struct slice {
         }
     }
 };
+
+// Columns of the second product that a thread works out at a time: four, where B's rows are whole groups of them on their boundaries.
+template<typename WT>
+__device__ __forceinline__ void load4(const WT *p, float (&w)[4]) {
+    if constexpr (sizeof(WT) == 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+        bf16x2_to_f32(v.x, w[0], w[1]);
+        bf16x2_to_f32(v.y, w[2], w[3]);
+    }
+}
 
 // A block takes p.block_rows rows, cut into parts by their lengths alone, and deals the parts to its warps, so that a long row
 // does not hold up the others.  A warp decodes 128 entries at a time into shared memory, {gene, value}, the next ones' indices and
@@ -261,20 +275,42 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
         *sum = h;
     }
     __syncthreads();
-    const int n = static_cast<int>(p.n);
-    for (int i = threadIdx.x; i < rows * n; i += kWarps * 32) {
-        const int r = i / n, c = i - r * n, a = row_adapter[r];
-        float v = 0.0f;
-        if (first_part[r] < first_part[r + 1]) {
-            const float *hidden = sums + first_part[r] * p.rank;
-            const WT *up = static_cast<const WT *>(p.up) + static_cast<std::int64_t>(a) * p.rank * n + c;
-#pragma unroll 8
-            for (int k = 0; k < p.rank; ++k) v = fmaf(hidden[k], load1(up + static_cast<std::int64_t>(k) * n), v);
-            v *= p.alpha * (p.scale != nullptr ? __ldg(p.scale + a) : 1.0f);
-        }
+    const int n = static_cast<int>(p.n), per_row = p.up_quads ? n >> 2 : n;
+    for (int i = threadIdx.x; i < rows * per_row; i += kWarps * 32) {
+        const int r = i / per_row, a = row_adapter[r];
+        const bool has = first_part[r] < first_part[r + 1];
+        const float *hidden = sums + first_part[r] * p.rank;
+        const float factor = has ? p.alpha * (p.scale != nullptr ? __ldg(p.scale + a) : 1.0f) : 0.0f;
+        const int c = p.up_quads ? i % per_row * 4 : i % per_row;
+        const WT *up = static_cast<const WT *>(p.up) + static_cast<std::int64_t>(has ? a : 0) * p.rank * n + c;
         float *out = p.out + (row0 + r) * p.out_ld + c;
-        if (p.beta != 0.0f) v = fmaf(p.beta, *out, v);
-        *out = finish_output(v, p.bias, c, p.epilogue);
+        if (p.up_quads) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (has) {
+#pragma unroll 8
+                for (int k = 0; k < p.rank; ++k, up += n) {
+                    float w[4];
+                    load4(up, w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = fmaf(hidden[k], w[j], v[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] *= factor;
+                if (p.beta != 0.0f) v[j] = fmaf(p.beta, out[j], v[j]);
+                out[j] = finish_output(v[j], p.bias, c + j, p.epilogue);
+            }
+        } else {
+            float v = 0.0f;
+            if (has) {
+#pragma unroll 8
+                for (int k = 0; k < p.rank; ++k, up += n) v = fmaf(hidden[k], load1(up), v);
+            }
+            v *= factor;
+            if (p.beta != 0.0f) v = fmaf(p.beta, *out, v);
+            *out = finish_output(v, p.bias, c, p.epilogue);
+        }
     }
 }
 
@@ -358,6 +394,8 @@ extern "C" cb200_status cb200_qcsr_adapters(const cb200_adapters *d, void *strea
         p.block_rows *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf16 = d->weight_dtype == CB200_DTYPE_BF16;
+    const std::uintptr_t quad = bf16 ? 8u : 16u;
+    p.up_quads = d->n % 4 == 0 && reinterpret_cast<std::uintptr_t>(d->up) % quad == 0u ? 1 : 0;
     if (x->bits == 8) return bf16 ? dispatch<8, __nv_bfloat16>(p, end - begin, s) : dispatch<8, float>(p, end - begin, s);
     return bf16 ? dispatch<4, __nv_bfloat16>(p, end - begin, s) : dispatch<4, float>(p, end - begin, s);
 }

@@ -174,6 +174,41 @@ def test_a_rows_bits_follow_from_the_row(cuda_device, oracle):
     assert torch.equal(ops.adapter_forward(to_dev(piece, cuda_device), adapter[20:33].contiguous(), down, up, scale), whole[20:33])
 
 
+@pytest.mark.parametrize("rows,genes,mean,rank,bits,dtype", [(2600, 2000, 900, 16, 8, torch.bfloat16), (1500, 33_538, 1500, 8, 4, torch.float32),
+                                                             (3000, 1500, 800, 5, 8, torch.float32), (2400, 3000, 1000, 128, 4, torch.bfloat16)])
+def test_large_batches(cuda_device, oracle, rows, genes, mean, rank, bits, dtype):
+    """Two million entries and more, whose scales (and, of 33,538 genes, some zero-points) are kept in shared memory: against the
+    definition on some rows, bit for bit what the same rows give in ranges of fewer entries, with empty rows by the hundred, rows
+    without an adapter and one row that holds every gene."""
+    rng = np.random.default_rng(rank)
+    lengths = np.minimum(rng.lognormal(np.log(mean), 0.6, rows).astype(np.int64), genes)
+    lengths[100:400] = 0
+    lengths[-1] = 0
+    lengths[500] = genes
+    row_ptr = np.concatenate([[0], np.cumsum(lengths)])
+    col = np.concatenate([np.sort(rng.permutation(genes)[:k]) for k in lengths]).astype(np.int32)
+    c = host_pack(oracle, dict(rows=rows, cols=genes, bits=bits, policy=1, row_ptr=row_ptr, col_idx=col, scales=rng.uniform(0.01, 0.5, genes).astype(np.float32),
+                               offsets=rng.uniform(-1, 1, genes).astype(np.float32), values=rng.uniform(-2, 40, len(col)).astype(np.float32)))
+    assert len(col) // rows * rows >= 2_000_000
+    x = to_dev(c, cuda_device)
+    n = 40
+    down, up, scale = weights(6, genes, rank, n, dtype, cuda_device, rank)
+    adapter = torch.from_numpy(rng.integers(-1, 6, rows)).int()
+    on_device = adapter.to(cuda_device)
+    whole = ops.adapter_forward(x, on_device, down, up, scale)
+    pieces = torch.full_like(whole, float("nan"))
+    bounds = np.linspace(0, rows, 6).astype(int)
+    for lo, hi in zip(bounds[:-1], bounds[1:]):
+        ops.adapter_forward(x, on_device, down, up, scale, out=pieces, row_begin=int(lo), row_end=int(hi))
+    assert torch.equal(whole, pieces)
+    some = np.concatenate([np.arange(90, 110), [399, 400, 500, rows - 1], rng.integers(0, rows, 20)])
+    for r in some:
+        piece = rows_of(c, int(r), int(r) + 1)
+        want, bound = expected(*decoded(oracle, piece), adapter[int(r):int(r) + 1], down, up, scale)
+        # rows of up to 33,538 entries: parts of 1,152, nine segments in turn, eight of them more than counted
+        assert_within(whole[int(r):int(r) + 1].cpu(), want, bound * ((166 + 8 * 128) / 166), name=str(r))
+
+
 def test_pitch_of_the_output(cuda_device, oracle):
     c = case(oracle, 25, 200, 50, 4, 1, 15)
     down, up, scale = weights(2, 200, 8, 30, torch.float32, cuda_device, 7)
