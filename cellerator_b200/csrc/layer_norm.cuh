@@ -11,9 +11,10 @@
 
 namespace cb200 {
 
-// Widths.  Up to kNarrowColumns a row belongs to a group of lanes of one warp; wider ones to a block, or to a cluster of up to
-// eight blocks, each with a slice of the columns.
+// Widths.  Up to kNarrowColumns a row belongs to a group of lanes of one warp, wider ones to a block.  Forward, the widest belong to a
+// cluster of eight blocks, each with a slice of the columns; backward, rows that no block holds are taken in two passes.
 constexpr int kNarrowColumns = 512;
+constexpr int kBlockColumns = 4608; // of a row that one block holds, backward
 constexpr std::int64_t kMostColumns = 65536;
 constexpr int kNarrowThreads = 256;
 constexpr int kNarrowItems = 4; // quads of a row that a lane holds
@@ -54,6 +55,12 @@ inline wide_shape wide_shape_of(std::int64_t columns) {
     s.threads = ((s.slice_quads + s.quads_per_thread - 1) / s.quads_per_thread + 31) / 32 * 32;
     return s;
 }
+
+// Backward pass of rows that no block holds (layer_norm_columns.cu): parts of the sums of dgamma and dbeta, bytes of the rows' sums,
+// launch.  p.partials (for the parts) and `sums` are the caller's; sums is needed where p.dx is.
+std::int64_t layer_norm_columns_parts(std::int64_t rows, std::int64_t columns);
+std::uint64_t layer_norm_columns_sums_bytes(std::int64_t rows, std::int64_t columns);
+cb200_status launch_layer_norm_columns(const layer_norm_params &p, float *sums, cudaStream_t stream);
 
 // Launches a kernel of a wide row as clusters.
 template<typename K>

@@ -9,12 +9,11 @@
 namespace cb200 {
 namespace {
 
-// Most blocks (narrow) or clusters (wide) of a launch: each leaves 2 x columns sums.
+// Most blocks of a launch: each leaves 2 x columns sums.
 // Quads of a row that a lane holds: two up to 256 columns, as it keeps two sums for each of its columns and 24 warps are to fit an SM.
 constexpr int back_items(std::int64_t columns) { return columns <= 256 ? 2 : 4; }
 constexpr int kNarrowBlocks = 3; // narrow: resident on an SM, with two quads a lane; one less with four
 constexpr int kNarrowParts = 148 * kNarrowBlocks;
-constexpr int kWideParts = 148 * 4;
 
 // u and h in place of x and dy of some quads of a row; dz u and dz added to what the thread keeps of their columns, h and h u to the
 // row's sums.  at: where the quads' gamma (and, beta_at further, beta) stand in shared memory.
@@ -135,128 +134,80 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
     }
 }
 
-// A block, or a cluster of blocks that take a slice of the columns each, per row; a thread keeps the sums of its columns from row
-// to row.  In a cluster the two sums of a row go round while the row before is written and the one behind is worked on.  gamma and
-// beta of the slice are in shared memory: the sums, two rows and the next one's values take the registers.
-template<int SX, int SG, bool HALVES, int QT, bool CLUSTER>
-__global__ void __launch_bounds__(wide_threads(QT)) layer_norm_back_wide_kernel(const layer_norm_params p) {
-    __shared__ wide_notes<2, CLUSTER> notes;
-    extern __shared__ __align__(16) float parameters[]; // gamma and beta of the block's quads, and a quad each for threads without
-    const int lane = threadIdx.x & 31, all_warps = p.cluster * (blockDim.x >> 5), n = p.columns;
-    const int rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
-    const std::int64_t first = CLUSTER ? blockIdx.x / p.cluster : blockIdx.x, stride = CLUSTER ? gridDim.x / p.cluster : gridDim.x;
+constexpr int kBlockQuads = 2, kBlockThreads = kBlockColumns / (4 * kBlockQuads); // of a thread; of a block, at most
+
+// A block per row; a thread keeps the sums of its columns from row to row.  gamma and beta are in shared memory: the sums, a row and
+// the next one's values take the registers.
+template<int SX, int SG, bool HALVES>
+__global__ void __launch_bounds__(kBlockThreads) layer_norm_back_block_kernel(const layer_norm_params p) {
+    constexpr int QT = kBlockQuads;
+    __shared__ float notes[2][2][kBlockThreads / 32]; // of two rows in turn: each warp's sums
+    extern __shared__ __align__(16) float parameters[]; // gamma and beta, and a quad each for threads without columns
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = p.columns, beta_at = ((n + 3) & ~3) + 4;
     const bool half = p.x.dtype == CB200_DTYPE_F16, half_dy = p.dy.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    const int beta_at = (p.slice_quads + 1) * 4, column0 = rank * p.slice_quads * 4;
     for (int c = threadIdx.x; c < beta_at; c += blockDim.x) {
-        const bool in = column0 + c < n && c < p.slice_quads * 4;
-        parameters[c] = p.gamma != nullptr && in ? __ldg(p.gamma + column0 + c) : 1.0f;
-        parameters[beta_at + c] = p.beta != nullptr && in ? __ldg(p.beta + column0 + c) : 0.0f;
+        parameters[c] = p.gamma != nullptr && c < n ? __ldg(p.gamma + c) : 1.0f;
+        parameters[beta_at + c] = p.beta != nullptr && c < n ? __ldg(p.beta + c) : 0.0f;
     }
     float dgamma[QT][4], dbeta[QT][4];
-    int col[QT], at[QT];
-    wide_columns<QT>(p, rank, col);
+    int col[QT];
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        at[i] = min(i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x), p.slice_quads) * 4;
+        col[i] = min((i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 4, (n + 3) & ~3);
 #pragma unroll
         for (int k = 0; k < 4; ++k) dgamma[i][k] = dbeta[i][k] = 0.0f;
     }
-    const int own = min(p.slice_quads * 4, n - column0); // columns of the block
     const float inverse = 1.0f / static_cast<float>(n);
     raw_quad<SX> raw_x[QT];
     raw_quad<SG> raw_dy[QT];
     float2 stats;
     const auto fetch = [&](std::int64_t row) {
         if (row >= p.rows) return;
-        if (threadIdx.x == 0 && row + stride < p.rows && own > 0) { // the row behind it, on its way to L2
-            prefetch_bytes(p.x.base + (row + stride) * p.x.pitch + column0 * SX, static_cast<std::uint32_t>(own) * SX);
-            prefetch_bytes(p.dy.base + (row + stride) * p.dy.pitch + column0 * SG, static_cast<std::uint32_t>(own) * SG);
-        }
         stats = *reinterpret_cast<const float2 *>(p.stats + 2 * row);
         load_quads(p.x.base + row * p.x.pitch, col, n, p.per_access, raw_x);
         load_quads(p.dy.base + row * p.dy.pitch, col, n, p.per_access, raw_dy);
     };
-    float x[QT][4], dy[QT][4]; // x and dy of a row, then its u and h
-    const auto widened = [&]() {
+    fetch(blockIdx.x);
+    __syncthreads();
+    int set = 0;
+    for (std::int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, set ^= 1) {
+        float x[QT][4], dy[QT][4], sums[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             raw_x[i].template widen<HALVES>(half, x[i]);
             raw_dy[i].template widen<HALVES>(half_dy, dy[i]);
         }
-    };
-    const auto summed = [&](std::int64_t row, float2 of_row, float (&sums)[2]) {
-        sums[0] = sums[1] = 0.0f;
+        const float mean = stats.x, rstd = stats.y;
+        fetch(row + gridDim.x);
         drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, dy);
-        const auto terms = [&](auto kind) { row_terms<decltype(kind)::value>(of_row.x, of_row.y, parameters, beta_at, at, x, dy, dgamma, dbeta, sums); };
+        const auto terms = [&](auto kind) { row_terms<decltype(kind)::value>(mean, rstd, parameters, beta_at, col, x, dy, dgamma, dbeta, sums); };
         if (p.epilogue == CB200_EPILOGUE_NONE) terms(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
         else if (p.epilogue == CB200_EPILOGUE_RELU) terms(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
         else if (p.epilogue == CB200_EPILOGUE_GELU_ERF) terms(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
         else terms(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
-        warp_sums<2>(sums);
-    };
-    const auto finish = [&](const float (&u)[QT][4], const float (&h)[QT][4], std::int64_t row, float rstd, int set) {
-        if (p.dx.base == nullptr) return;
-        float sums[2] = {0.0f, 0.0f};
-        for (int w = lane; w < all_warps; w += 32) {
-            sums[0] += notes.note[set][w][0];
-            sums[1] += notes.note[set][w][1];
+        if (p.dx.base == nullptr) continue;
+        warp_sums(sums);
+        if (lane == 0) {
+            notes[set][0][warp] = sums[0];
+            notes[set][1][warp] = sums[1];
         }
-        warp_sums<2>(sums);
+        __syncthreads();
+        sums[0] = lane < warps ? notes[set][0][lane] : 0.0f;
+        sums[1] = lane < warps ? notes[set][1][lane] : 0.0f;
+        warp_sums(sums);
         sums[0] *= inverse;
         sums[1] *= inverse;
-        float v[QT][4];
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = rstd * (h[i][k] - sums[0] - u[i][k] * sums[1]);
+            for (int k = 0; k < 4; ++k) x[i][k] = rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
         }
-        store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, n, p.per_access, p.dx.dtype, v);
-    };
-    fetch(first);
-    __syncthreads();
-    int set = 0;
-    float sums[2];
-    if constexpr (CLUSTER) {
-        float u[QT][4], h[QT][4], rstd = 0.0f; // of the row before
-        cluster_arrive();                      // every block of the cluster has begun
-        std::int64_t row = first;
-        for (; row < p.rows; row += stride) {
-            widened();
-            const float2 of_row = stats;
-            summed(row, of_row, sums);
-            cluster_wait();
-            notes.leave(sums, set, rank, p.cluster);
-            cluster_arrive();
-            fetch(row + stride);
-            if (row != first) finish(u, h, row - stride, rstd, set == 0 ? 2 : set - 1);
-            set = next_set(set, 3);
-            rstd = of_row.y;
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    u[i][k] = x[i][k];
-                    h[i][k] = dy[i][k];
-                }
-            }
-        }
-        cluster_wait();
-        if (row != first) finish(u, h, row - stride, rstd, set == 0 ? 2 : set - 1);
-    } else {
-        for (std::int64_t row = first; row < p.rows; row += stride, set ^= 1) {
-            widened();
-            const float2 of_row = stats;
-            fetch(row + stride);
-            summed(row, of_row, sums);
-            notes.leave(sums, set, rank, p.cluster);
-            __syncthreads();
-            finish(x, dy, row, of_row.y, set);
-        }
+        store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, n, p.per_access, p.dx.dtype, x);
     }
     let_next_launch_start();
     if (p.partials == nullptr) return;
-    float *out = p.partials + first * 2 * n;
+    float *out = p.partials + static_cast<std::int64_t>(blockIdx.x) * 2 * n;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
 #pragma unroll
@@ -295,6 +246,10 @@ std::int64_t narrow_parts(std::int64_t rows, std::int64_t columns) {
     return std::min<std::int64_t>((rows + per_block - 1) / per_block, back_items(columns) == 2 ? kNarrowParts : kNarrowParts / kNarrowBlocks * (kNarrowBlocks - 1));
 }
 
+// Threads of a block of a row that it holds, and blocks of a launch: those that are resident with 96 registers a thread.
+int block_threads(std::int64_t columns) { return static_cast<int>((columns + 4 * kBlockQuads * 32 - 1) / (4 * kBlockQuads * 32) * 32); }
+std::int64_t block_parts(std::int64_t rows, std::int64_t columns) { return std::min<std::int64_t>(rows, 148 * std::max(1, 640 / block_threads(columns))); }
+
 struct backward_launch {
     layer_norm_params p;
     float *dgamma, *dbeta;
@@ -304,19 +259,14 @@ struct backward_launch {
     cb200_status finish(std::int64_t parts) const {
         count_launch();
         CB200_CUDA_OK(cudaGetLastError());
+        return meet(parts);
+    }
+    cb200_status meet(std::int64_t parts) const {
         if (p.partials == nullptr) return CB200_STATUS_SUCCESS;
         CB200_CUDA_OK(launch_kernel(true, layer_norm_meet_kernel, dim3(static_cast<unsigned>((2 * p.columns + 31) / 32)), kMeetWarps * 32, 0, stream,
                                     static_cast<const float *>(p.partials), static_cast<int>(parts), p.columns, dgamma, dbeta));
         count_launch();
         return CB200_STATUS_SUCCESS;
-    }
-    template<auto kernel>
-    cb200_status wide(const wide_shape &shape) const {
-        const std::size_t smem = static_cast<std::size_t>(shape.slice_quads + 1) * 32u; // up to 37 KB with two quads to a thread, 66 KB with four
-        if (shape.quads_per_thread != 2) CB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 66 * 1024));
-        const std::int64_t parts = std::min<std::int64_t>({p.rows, kWideParts / shape.cluster, resident_clusters<kernel>(shape, smem, device)});
-        CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(parts), smem, stream));
-        return finish(parts);
     }
     template<int SX, int SG, bool HALVES, int KIND>
     cb200_status run() {
@@ -327,19 +277,20 @@ struct backward_launch {
             else layer_norm_back_narrow_kernel<SX, SG, HALVES, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             return finish(parts);
         }
-        const wide_shape shape = wide_shape_of(p.columns);
-        p.cluster = shape.cluster;
-        p.slice_quads = shape.slice_quads;
-        if (shape.cluster == 1) return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 2, false>>(shape);
-        if (shape.quads_per_thread == 2) return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 2, true>>(shape);
-        return wide<layer_norm_back_wide_kernel<SX, SG, HALVES, 4, true>>(shape);
+        const std::int64_t parts = block_parts(p.rows, p.columns);
+        const std::size_t smem = static_cast<std::size_t>((p.columns + 3) / 4 + 1) * 32u;
+        layer_norm_back_block_kernel<SX, SG, HALVES><<<static_cast<unsigned>(parts), block_threads(p.columns), smem, stream>>>(p);
+        return finish(parts);
     }
 };
 
 std::uint64_t partial_bytes(std::int64_t rows, std::int64_t columns) {
-    const std::int64_t parts = columns <= kNarrowColumns ? narrow_parts(rows, columns) : std::min<std::int64_t>(rows, kWideParts / wide_shape_of(columns).cluster);
+    const std::int64_t parts = columns <= kNarrowColumns ? narrow_parts(rows, columns)
+                               : columns <= kBlockColumns ? block_parts(rows, columns)
+                                                          : layer_norm_columns_parts(rows, columns);
     return static_cast<std::uint64_t>(parts) * 2u * static_cast<std::uint64_t>(columns) * sizeof(float);
 }
+std::uint64_t sums_bytes(std::int64_t rows, std::int64_t columns) { return columns <= kBlockColumns ? 0u : layer_norm_columns_sums_bytes(rows, columns); }
 
 } // namespace
 } // namespace cb200
@@ -350,7 +301,7 @@ extern "C" cb200_status cb200_layer_norm_backward_workspace(int64_t rows, int64_
     if (bytes == nullptr) return fail(CB200_STATUS_INVALID_ARGUMENT, "workspace needs an output");
     if (rows < 0 || columns < 1 || columns > kMostColumns || rows >= (1ll << 32))
         return fail(CB200_STATUS_INVALID_SHAPE, "the layer norm takes fewer than 2^32 rows of 1 to %lld columns, got %lld x %lld", (long long)kMostColumns, (long long)rows, (long long)columns);
-    *bytes = partial_bytes(rows, columns);
+    *bytes = rows == 0 ? 0u : partial_bytes(rows, columns) + sums_bytes(rows, columns);
     return CB200_STATUS_SUCCESS;
 }
 
@@ -368,12 +319,15 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
         return fail(CB200_STATUS_INVALID_ARGUMENT, "dx overlaps x or dy without being it");
     if (d->dgamma != nullptr && d->dgamma == d->dbeta) return fail(CB200_STATUS_INVALID_ARGUMENT, "dgamma and dbeta are the same vector");
     const bool sums = d->dgamma != nullptr || d->dbeta != nullptr;
-    if (sums && p.rows > 0) {
-        const std::uint64_t need = partial_bytes(p.rows, p.columns);
+    const bool two_passes = p.columns > kBlockColumns && p.dx.base != nullptr;
+    float *row_sums = nullptr;
+    if ((sums || two_passes) && p.rows > 0) {
+        const std::uint64_t partial = sums ? partial_bytes(p.rows, p.columns) : 0u, need = partial + (two_passes ? sums_bytes(p.rows, p.columns) : 0u);
         if (d->workspace == nullptr || d->workspace_bytes < need || reinterpret_cast<std::uintptr_t>(d->workspace) % 4u != 0u)
             return fail(CB200_STATUS_INSUFFICIENT_WORKSPACE, "workspace of %llu bytes needed, %llu given", (unsigned long long)need,
                         (unsigned long long)(d->workspace == nullptr ? 0u : d->workspace_bytes));
-        p.partials = static_cast<float *>(d->workspace);
+        if (sums) p.partials = static_cast<float *>(d->workspace);
+        row_sums = reinterpret_cast<float *>(static_cast<unsigned char *>(d->workspace) + partial);
     }
     p.per_access = columns_per_access(p.dy, p.per_access);
     if (p.dx.base != nullptr) p.per_access = columns_per_access(p.dx, p.per_access);
@@ -389,6 +343,10 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
         return CB200_STATUS_SUCCESS;
     }
     if (!sums && p.dx.base == nullptr) return CB200_STATUS_SUCCESS;
+    if (p.columns > kBlockColumns) {
+        st = launch_layer_norm_columns(p, row_sums, b.stream);
+        return st == CB200_STATUS_SUCCESS ? b.meet(layer_norm_columns_parts(p.rows, p.columns)) : st;
+    }
     const bool wide_x = element_bytes(p.x.dtype) == 4, wide_dy = element_bytes(p.dy.dtype) == 4;
     return with_epilogue(p.epilogue, [&](auto kind) {
         const auto of_sizes = [&](auto halves) {

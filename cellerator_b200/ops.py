@@ -606,7 +606,7 @@ def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, 
         dbeta = torch.empty_like(beta)
     dgamma_ptr, dbeta_ptr = _vector(dgamma, "dgamma", columns), _vector(dbeta, "dbeta", columns)
     workspace_ptr = workspace_bytes = 0
-    if workspace is None and (dgamma_ptr or dbeta_ptr) and rows:
+    if workspace is None and rows:
         workspace = stats.new_empty(layer_norm_backward_workspace(rows, columns) // 4)
     if workspace is not None:
         workspace_ptr, workspace_bytes = workspace.data_ptr(), workspace.nbytes

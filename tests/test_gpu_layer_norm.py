@@ -246,6 +246,40 @@ def test_rows_do_not_depend_on_their_neighbours(cuda_device):
             assert torch.equal(ops.layer_norm_backward(x[lo:hi], dy[lo:hi], stats[lo:hi].contiguous(), gamma, beta, first_row=lo, **kw)[0], grads[0][lo:hi])
 
 
+@pytest.mark.parametrize("cols", [300, 3000, 5001, 40_000])
+def test_some_of_the_gradients(cuda_device, cols):
+    """Each gradient alone through the C entry has the bits of all together, and the others' memory is left as it was."""
+    import ctypes as C
+    from cellerator_b200 import capi
+    rows = 90
+    x, dy = matrix(rows, cols, torch.float32, cuda_device, 123), matrix(rows, cols, torch.float32, cuda_device, 124)
+    gamma, beta = parameters(cols, cuda_device, 125)
+    stats = torch.empty(rows, 2, device=cuda_device)
+    ops.layer_norm(x, gamma, beta, stats=stats)
+    want = ops.layer_norm_backward(x, dy, stats, gamma, beta, epilogue="gelu_erf")
+    workspace = torch.empty(ops.layer_norm_backward_workspace(rows, cols), dtype=torch.uint8, device=cuda_device)
+    for asked in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (False, False, False)):
+        got = [torch.full_like(t, 7.0) for t in want]
+        n = capi.header(capi.LayerNorm())
+        n.rows, n.columns, n.x, n.x_ld, n.dy, n.dy_ld, n.dx_ld = rows, cols, x.data_ptr(), cols, dy.data_ptr(), cols, cols
+        n.x_dtype = n.dy_dtype = n.dx_dtype = capi.DTYPE_F32
+        n.gamma, n.beta, n.stats, n.epilogue, n.device = gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), capi.EPILOGUE["gelu_erf"], cuda_device.index
+        n.dx, n.dgamma, n.dbeta = (t.data_ptr() if a else None for t, a in zip(got, asked))
+        if any(asked[1:]) or (asked[0] and cols > 4608):
+            n.workspace, n.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        capi.check(capi.lib().cb200_layer_norm_backward(C.byref(n), torch.cuda.current_stream(cuda_device).cuda_stream))
+        for g, w, a in zip(got, want, asked):
+            assert torch.equal(g, w if a else torch.full_like(w, 7.0))
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [(20_000, 5000, torch.bfloat16), (2700, 33_538, torch.float32)])
+def test_parts_of_many_rows(cuda_device, rows, cols, dtype):
+    """Parts of more rows than are taken at a time: sums of 64 rows on top of each other, 64 + 3 + 8 + 16 roundings of the bound's 96."""
+    x, dy = matrix(rows, cols, dtype, cuda_device, 133), matrix(rows, cols, dtype, cuda_device, 134)
+    gamma, beta = parameters(cols, cuda_device, 135)
+    check_backward(x, dy, gamma, beta, kind="gelu_tanh", p=0.1)
+
+
 def test_graph_replay_on_another_stream(cuda_device):
     """Forward and backward captured together, eager calls in between; new inputs and a new mask at each replay."""
     for cols in (48, 5000):

@@ -133,7 +133,8 @@ def test_layer_norm_forward_refuses(change, status):
     (dict(dy=None), capi.INVALID_ARGUMENT), (dict(dy_ld=3), capi.INVALID_SHAPE), (dict(stats=None), capi.INVALID_ARGUMENT),
     (dict(dx=ADDRESS + 16), capi.INVALID_ARGUMENT), (dict(dx=3 * ADDRESS + 16), capi.INVALID_ARGUMENT), (dict(dx_dtype=0), capi.UNSUPPORTED),
     (dict(workspace=None), capi.INSUFFICIENT_WORKSPACE), (dict(workspace_bytes=3), capi.INSUFFICIENT_WORKSPACE),
-    (dict(workspace=ADDRESS + 2), capi.INSUFFICIENT_WORKSPACE), (dict(dgamma=ADDRESS * 9, dbeta=ADDRESS * 9), capi.INVALID_ARGUMENT),
+    (dict(workspace=ADDRESS + 2), capi.INSUFFICIENT_WORKSPACE),
+    (dict(columns=5000, x_ld=5000, dy_ld=5000, dx_ld=5000, dx=ADDRESS, dgamma=None, dbeta=None, workspace=None), capi.INSUFFICIENT_WORKSPACE), (dict(dgamma=ADDRESS * 9, dbeta=ADDRESS * 9), capi.INVALID_ARGUMENT),
 ])
 def test_layer_norm_backward_refuses(change, status):
     assert capi.lib().cb200_layer_norm_backward(C.byref(norm(**change)), None) == status
