@@ -172,11 +172,11 @@ __device__ __forceinline__ void load_parameters(const float *v, int col, int n, 
     for (int k = 0; k < 4; ++k) out[k] = v != nullptr && col + k < n ? __ldg(v + col + k) : otherwise;
 }
 
-// e^t and 1 / t by the hardware's approximations: e^t within 2 + 1.2 |t| units of the last place, 1 / t within one; what is too
-// small for a normal number is 0.
-__device__ __forceinline__ float fast_exp(float t) {
+// 2^t and 1 / t by the hardware's approximations, within 2 units and 1 unit of the last place; what is too small for a normal number
+// is 0.
+__device__ __forceinline__ float fast_exp2(float t) {
     float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     return e;
 }
 __device__ __forceinline__ float fast_reciprocal(float t) {
@@ -184,15 +184,19 @@ __device__ __forceinline__ float fast_reciprocal(float t) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
     return r;
 }
-// Logistic function: 1 / (1 + e^-t), within a few units of the last place of 1.
-__device__ __forceinline__ float logistic(float t) { return fast_reciprocal(1.0f + fast_exp(-t)); }
+// The factor of the tanh form of GELU, (1 + tanh(c (z + 0.044715 z^3))) / 2 with c = sqrt(2 / pi): the logistic function of twice that
+// argument, within a few units of the last place of 1.  zz: z^2, which may be cut off above 10^6 (the factor is 0 or 1 long before).
+__device__ __forceinline__ float tanh_gate(float z, float zz) {
+    // -2 c / ln 2 and 0.044715 of it
+    return fast_reciprocal(1.0f + fast_exp2(z * fmaf(-0.10294324f, zz, -2.3022082f)));
+}
 
-// act(z).  The tanh form of GELU, z / 2 (1 + tanh(c (z + 0.044715 z^3))), is z times the logistic function of twice that argument.
+// act(z)
 template<int KIND>
 __device__ __forceinline__ float activation(float z) {
     if constexpr (KIND == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
     if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return z * logistic(1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f));
+    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return z * tanh_gate(z, fminf(z * z, 1e6f));
     return z;
 }
 
@@ -201,11 +205,11 @@ template<int KIND>
 __device__ __forceinline__ float through_activation(float dy, float z) {
     if constexpr (KIND == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
     if constexpr (KIND == CB200_EPILOGUE_GELU_ERF)
-        return dy * fmaf(z, 0.39894228040143268f * fast_exp(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+        return dy * fmaf(z, 0.39894228f * fast_exp2(-0.72134752f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
     if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) {
-        const float zz = z * z, gate = logistic(1.5957691216057308f * z * fmaf(0.044715f, zz, 1.0f));
-        const float steep = gate * (1.0f - gate); // 0 far from 0, where the polynomial may be infinite
-        return dy * (steep > 0.0f ? fmaf(z * steep, 1.5957691216057308f * fmaf(0.134145f, zz, 1.0f), gate) : gate);
+        const float zz = fminf(z * z, 1e6f), gate = tanh_gate(z, zz);
+        const float steep = fmaf(-gate, gate, gate); // gate (1 - gate): 0 far from 0, times finite numbers
+        return dy * fmaf(z * steep, fmaf(0.21406445f, zz, 1.5957691f), gate); // 2 c and 3 times 0.044715 of it
     }
     return dy;
 }

@@ -219,26 +219,27 @@ __global__ void __launch_bounds__(kBlockThreads) layer_norm_back_block_kernel(co
     }
 }
 
-constexpr int kMeetWarps = 16;
+constexpr int kMeetWarps = 32; // most warps of a block
 
-// dgamma and dbeta from the parts' sums: a warp adds up every sixteenth part of 32 columns, then the warps' sums in order.
+// dgamma and dbeta from the parts' sums: of 32 columns, each warp adds up every so many parts, then the warps' sums in order.
 __global__ void __launch_bounds__(kMeetWarps * 32) layer_norm_meet_kernel(const float *partials, int parts, int columns, float *dgamma, float *dbeta) {
     __shared__ float meet[kMeetWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, c = blockIdx.x * 32 + lane;
     wait_for_previous_launch();
     float v = 0.0f;
     if (c < 2 * columns) {
-#pragma unroll 4
-        for (int part = warp; part < parts; part += kMeetWarps) v += partials[static_cast<std::int64_t>(part) * 2 * columns + c];
+#pragma unroll 16
+        for (int part = warp; part < parts; part += warps) v += partials[static_cast<std::int64_t>(part) * 2 * columns + c];
     }
     meet[warp][lane] = v;
     __syncthreads();
     if (warp != 0 || c >= 2 * columns) return;
-#pragma unroll
-    for (int w = 1; w < kMeetWarps; ++w) v += meet[w][lane];
+    for (int w = 1; w < warps; ++w) v += meet[w][lane];
     float *out = c < columns ? dgamma : dbeta;
     if (out != nullptr) out[c < columns ? c : c - columns] = v;
 }
+// Warps of a block: about twelve parts for each, so that a thread has its loads in flight at once.
+int meet_warps(std::int64_t parts) { return static_cast<int>(std::min<std::int64_t>(kMeetWarps, (parts + 11) / 12)); }
 
 // Blocks of a launch over narrow rows.
 std::int64_t narrow_parts(std::int64_t rows, std::int64_t columns) {
@@ -263,7 +264,7 @@ struct backward_launch {
     }
     cb200_status meet(std::int64_t parts) const {
         if (p.partials == nullptr) return CB200_STATUS_SUCCESS;
-        CB200_CUDA_OK(launch_kernel(true, layer_norm_meet_kernel, dim3(static_cast<unsigned>((2 * p.columns + 31) / 32)), kMeetWarps * 32, 0, stream,
+        CB200_CUDA_OK(launch_kernel(true, layer_norm_meet_kernel, dim3(static_cast<unsigned>((2 * p.columns + 31) / 32)), meet_warps(parts) * 32, 0, stream,
                                     static_cast<const float *>(p.partials), static_cast<int>(parts), p.columns, dgamma, dbeta));
         count_launch();
         return CB200_STATUS_SUCCESS;

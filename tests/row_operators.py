@@ -84,7 +84,7 @@ def norm_backward(x, dy, stats, gamma, beta, kind, factor):
     u has two roundings, z two more.  A slope is off by 20 U (1 + |z|) (as above) and, by gelu's second derivative < 1, the error of
     z.  Sums of a row have, of their magnitudes, 32 roundings as in norm_forward, or, piece by piece of 4,096 columns, 16 values of a
     thread, 5 shuffles, 8 warps and 16 pieces, 45, and one of the mean; sums over the rows of a test, one thread's rows, 5 shuffles,
-    8 warps, every 16th part and 16 of these, at most 96."""
+    8 warps, every so many parts (14 of them) and 32 of these, at most 96."""
     mean, rstd = stats[:, :1], stats[:, 1:]
     u = (x - mean) * rstd
     z = u * gamma + beta
