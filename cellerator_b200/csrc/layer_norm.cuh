@@ -11,13 +11,11 @@
 
 namespace cb200 {
 
-// Widths.  Up to kNarrowColumns a row belongs to a group of lanes of one warp, wider ones to a block.  Forward, the widest belong to a
+// Widths.  Up to 1,024 columns (backward 512) a row belongs to a group of lanes of one warp, wider ones to a block.  Forward, the widest belong to a
 // cluster of eight blocks, each with a slice of the columns; backward, rows that no block holds are taken in two passes.
-constexpr int kNarrowColumns = 512;
 constexpr int kBlockColumns = 4608; // of a row that one block holds, backward
 constexpr std::int64_t kMostColumns = 65536;
 constexpr int kNarrowThreads = 256;
-constexpr int kNarrowItems = 4; // quads of a row that a lane holds
 // Most threads of a block of a wide row, by the quads of a thread: eight blocks hold 36,864 columns with two, all 65,536 with four.
 constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 2 ? 576 : 512; }
 constexpr int kMostWarps = 18;
@@ -117,12 +115,21 @@ unsigned resident_clusters(const wide_shape &shape, std::size_t smem, int device
     return static_cast<unsigned>(found);
 }
 
-// Lanes of a narrow row, with `items` quads to a lane: as few as hold it, so that its sums take few shuffles.
-inline int narrow_lanes(std::int64_t columns, int items) {
+// How a narrow row is laid over the lanes of a warp: a power of two of them, with so many quads each that few are left empty (an
+// empty quad costs what a full one does: 8 columns with GELU and dropout took 211 us with four quads to a lane, 112 with two), and
+// of equal choices the first of `items`.
+struct narrow_shape {
+    int items, lanes;
+};
+inline narrow_shape narrow_shape_of(std::int64_t columns, const int *items, int choices) {
     const std::int64_t quads = (columns + 3) / 4;
-    int lanes = 1;
-    while (lanes < 32 && lanes * items < quads) lanes *= 2;
-    return lanes;
+    narrow_shape best{0, 0};
+    for (int i = 0; i < choices; ++i) {
+        int lanes = 1;
+        while (lanes < 32 && lanes * items[i] < quads) lanes *= 2;
+        if (lanes * items[i] >= quads && (best.lanes == 0 || lanes * items[i] < best.lanes * best.items)) best = narrow_shape{items[i], lanes};
+    }
+    return best;
 }
 
 inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward, layer_norm_params *p) {
@@ -148,21 +155,9 @@ inline cb200_status layer_norm_checked(const cb200_layer_norm *d, bool backward,
     p->columns = static_cast<int>(d->columns);
     p->epilogue = d->epilogue;
     p->epsilon = d->epsilon;
-    p->lanes = narrow_lanes(d->columns, kNarrowItems);
     p->per_access = columns_per_access(p->x, columns_of_access(d->columns));
     if (!backward && !(d->epsilon >= 0.0f && d->epsilon < 3.4e38f)) return fail(CB200_STATUS_INVALID_ARGUMENT, "epsilon %g is no number from 0 on", d->epsilon);
     return CB200_STATUS_SUCCESS;
-}
-
-// Calls f with the epilogue as a constant.
-template<typename F>
-cb200_status with_epilogue(int kind, F f) {
-    switch (kind) {
-    case CB200_EPILOGUE_RELU: return f(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
-    case CB200_EPILOGUE_GELU_ERF: return f(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
-    case CB200_EPILOGUE_GELU_TANH: return f(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
-    default: return f(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
-    }
 }
 
 #if defined(__CUDACC__)
@@ -240,6 +235,14 @@ __device__ __forceinline__ void through_as(float (&dy)[Q][4], const float (&u)[Q
         dy[i][2] = through_activation<KIND>(dy[i][2], fmaf(u[i][2], gamma[i].z, beta[i].z));
         dy[i][3] = through_activation<KIND>(dy[i][3], fmaf(u[i][3], gamma[i].w, beta[i].w));
     }
+}
+// Calls f with the epilogue as a constant: one branch for all that f does.
+template<typename F>
+__device__ __forceinline__ void with_epilogue(int kind, F f) {
+    if (kind == CB200_EPILOGUE_NONE) f(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
+    else if (kind == CB200_EPILOGUE_RELU) f(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
+    else if (kind == CB200_EPILOGUE_GELU_ERF) f(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
+    else f(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
 }
 template<int Q>
 __device__ __forceinline__ void drop_quads(const dropout_args &d, std::uint64_t sequence, std::uint32_t row, const int (&col)[Q], float (&v)[Q][4]) {

@@ -10,10 +10,10 @@ namespace cb200 {
 namespace {
 
 // Most blocks of a launch: each leaves 2 x columns sums.
-// Quads of a row that a lane holds: two up to 256 columns, as it keeps two sums for each of its columns and 24 warps are to fit an SM.
-constexpr int back_items(std::int64_t columns) { return columns <= 256 ? 2 : 4; }
-constexpr int kNarrowBlocks = 3; // narrow: resident on an SM, with two quads a lane; one less with four
-constexpr int kNarrowParts = 148 * kNarrowBlocks;
+constexpr int kNarrowItems[] = {2, 4, 3}; // quads of a row that a lane can hold, two by preference (64 columns: 97 us, four 122)
+constexpr std::int64_t kNarrowColumns = 4 * 32 * 4;
+// Blocks that are resident on an SM: with two quads to a lane, which keeps two sums for each of its columns, 24 warps fit.
+constexpr int narrow_blocks(int items) { return items == 2 ? 3 : 2; }
 
 // u and h in place of x and dy of some quads of a row; dz u and dz added to what the thread keeps of their columns, h and h u to the
 // row's sums.  at: where the quads' gamma (and, beta_at further, beta) stand in shared memory.
@@ -49,8 +49,8 @@ __device__ __forceinline__ void row_terms(float mean, float rstd, const float *g
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  Columns past the last hold
 // zeros in dy, so that they add nothing.
-template<int SX, int SG, bool HALVES, int KIND, int ITEMS>
-__global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : kNarrowBlocks - 1) layer_norm_back_narrow_kernel(const layer_norm_params p) {
+template<int SX, int SG, bool HALVES, int ITEMS>
+__global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? 3 : 2) layer_norm_back_narrow_kernel(const layer_norm_params p) {
     __shared__ float meet[kNarrowThreads / 32][ITEMS * 4 * 32];
     constexpr int kParameters = ITEMS * 4 * 32 + 4;
     __shared__ __align__(16) float parameters[2][kParameters]; // gamma and beta: registers are short here
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? kNarrowBlocks : k
         fetch(row + step);
         if (active) {
             drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, dy);
-            row_terms<KIND>(mean, rstd, parameters[0], kParameters, col, x, dy, dgamma, dbeta, sums);
+            with_epilogue(p.epilogue, [&](auto kind) { row_terms<decltype(kind)::value>(mean, rstd, parameters[0], kParameters, col, x, dy, dgamma, dbeta, sums); });
         }
         lane_sums(sums, p.lanes);
         sums[0] *= inverse;
@@ -181,11 +181,7 @@ __global__ void __launch_bounds__(kBlockThreads) layer_norm_back_block_kernel(co
         const float mean = stats.x, rstd = stats.y;
         fetch(row + gridDim.x);
         drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, dy);
-        const auto terms = [&](auto kind) { row_terms<decltype(kind)::value>(mean, rstd, parameters, beta_at, col, x, dy, dgamma, dbeta, sums); };
-        if (p.epilogue == CB200_EPILOGUE_NONE) terms(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
-        else if (p.epilogue == CB200_EPILOGUE_RELU) terms(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
-        else if (p.epilogue == CB200_EPILOGUE_GELU_ERF) terms(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
-        else terms(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
+        with_epilogue(p.epilogue, [&](auto kind) { row_terms<decltype(kind)::value>(mean, rstd, parameters, beta_at, col, x, dy, dgamma, dbeta, sums); });
         if (p.dx.base == nullptr) continue;
         warp_sums(sums);
         if (lane == 0) {
@@ -243,8 +239,9 @@ int meet_warps(std::int64_t parts) { return static_cast<int>(std::min<std::int64
 
 // Blocks of a launch over narrow rows.
 std::int64_t narrow_parts(std::int64_t rows, std::int64_t columns) {
-    const std::int64_t per_block = kNarrowThreads / narrow_lanes(columns, back_items(columns));
-    return std::min<std::int64_t>((rows + per_block - 1) / per_block, back_items(columns) == 2 ? kNarrowParts : kNarrowParts / kNarrowBlocks * (kNarrowBlocks - 1));
+    const narrow_shape narrow = narrow_shape_of(columns, kNarrowItems, 3);
+    const std::int64_t per_block = kNarrowThreads / narrow.lanes;
+    return std::min<std::int64_t>((rows + per_block - 1) / per_block, 148 * narrow_blocks(narrow.items));
 }
 
 // Threads of a block of a row that it holds, and blocks of a launch: those that are resident with 96 registers a thread.
@@ -269,13 +266,15 @@ struct backward_launch {
         count_launch();
         return CB200_STATUS_SUCCESS;
     }
-    template<int SX, int SG, bool HALVES, int KIND>
+    template<int SX, int SG, bool HALVES>
     cb200_status run() {
         if (p.columns <= kNarrowColumns) {
             const std::int64_t parts = narrow_parts(p.rows, p.columns);
-            p.lanes = narrow_lanes(p.columns, back_items(p.columns));
-            if (back_items(p.columns) == 2) layer_norm_back_narrow_kernel<SX, SG, HALVES, KIND, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
-            else layer_norm_back_narrow_kernel<SX, SG, HALVES, KIND, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            const narrow_shape narrow = narrow_shape_of(p.columns, kNarrowItems, 3);
+            p.lanes = narrow.lanes;
+            if (narrow.items == 2) layer_norm_back_narrow_kernel<SX, SG, HALVES, 2><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            else if (narrow.items == 3) layer_norm_back_narrow_kernel<SX, SG, HALVES, 3><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
+            else layer_norm_back_narrow_kernel<SX, SG, HALVES, 4><<<static_cast<unsigned>(parts), kNarrowThreads, 0, stream>>>(p);
             return finish(parts);
         }
         const std::int64_t parts = block_parts(p.rows, p.columns);
@@ -349,13 +348,11 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
         return st == CB200_STATUS_SUCCESS ? b.meet(layer_norm_columns_parts(p.rows, p.columns)) : st;
     }
     const bool wide_x = element_bytes(p.x.dtype) == 4, wide_dy = element_bytes(p.dy.dtype) == 4;
-    return with_epilogue(p.epilogue, [&](auto kind) {
-        const auto of_sizes = [&](auto halves) {
-            constexpr bool H = decltype(halves)::value;
-            if (wide_x) return wide_dy ? b.run<4, 4, H, kind()>() : b.run<4, 2, H, kind()>();
-            return wide_dy ? b.run<2, 4, H, kind()>() : b.run<2, 2, H, kind()>();
-        };
-        return p.x.dtype == CB200_DTYPE_F16 || p.dy.dtype == CB200_DTYPE_F16 || (p.dx.base != nullptr && p.dx.dtype == CB200_DTYPE_F16) ? of_sizes(std::true_type{})
-                                                                                                                                        : of_sizes(std::false_type{});
-    });
+    const auto of_sizes = [&](auto halves) {
+        constexpr bool H = decltype(halves)::value;
+        if (wide_x) return wide_dy ? b.run<4, 4, H>() : b.run<4, 2, H>();
+        return wide_dy ? b.run<2, 4, H>() : b.run<2, 2, H>();
+    };
+    return p.x.dtype == CB200_DTYPE_F16 || p.dy.dtype == CB200_DTYPE_F16 || (p.dx.base != nullptr && p.dx.dtype == CB200_DTYPE_F16) ? of_sizes(std::true_type{})
+                                                                                                                                    : of_sizes(std::false_type{});
 }

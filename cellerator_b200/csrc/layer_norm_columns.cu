@@ -81,10 +81,7 @@ __global__ void __launch_bounds__(kSumThreads) layer_norm_sums_kernel(const colu
                 add_terms<decltype(kind)::value>(u, dz, gamma, beta, sums[2 * r], sums[2 * r + 1]);
             }
         };
-        if (p.epilogue == CB200_EPILOGUE_NONE) rows(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
-        else if (p.epilogue == CB200_EPILOGUE_RELU) rows(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
-        else if (p.epilogue == CB200_EPILOGUE_GELU_ERF) rows(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
-        else rows(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
+        with_epilogue(p.epilogue, rows);
     }
     let_next_launch_start();
     warp_sums(sums);
@@ -165,10 +162,7 @@ __global__ void __launch_bounds__(kColumnThreads) layer_norm_columns_kernel(cons
                     if (p.dx.base != nullptr) store_quads<HALVES>(p.dx.base + (row0 + first + r) * p.dx.pitch, col, n, p.per_access, p.dx.dtype, dx);
                 }
             };
-            if (p.epilogue == CB200_EPILOGUE_NONE) some(std::integral_constant<int, CB200_EPILOGUE_NONE>{});
-            else if (p.epilogue == CB200_EPILOGUE_RELU) some(std::integral_constant<int, CB200_EPILOGUE_RELU>{});
-            else if (p.epilogue == CB200_EPILOGUE_GELU_ERF) some(std::integral_constant<int, CB200_EPILOGUE_GELU_ERF>{});
-            else some(std::integral_constant<int, CB200_EPILOGUE_GELU_TANH>{});
+            with_epilogue(p.epilogue, some);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {

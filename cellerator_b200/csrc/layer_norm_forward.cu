@@ -7,33 +7,37 @@
 namespace cb200 {
 namespace {
 
-constexpr int kNarrowBlocks = 3; // resident on an SM
+constexpr int kNarrowItems[] = {4, 3, 2, 6, 8}; // quads of a row that a lane can hold, four by preference (32 columns: 65 us, eight 111)
+constexpr std::int64_t kNarrowColumns = 8 * 32 * 4;
+// Blocks that are resident on an SM.
+constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
-// shared memory: a lane's sixteen columns of them would take a third of its registers.
-template<int SIZE, bool HALVES, int KIND>
-__global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narrow_kernel(const layer_norm_params p) {
-    __shared__ __align__(16) float parameters[2][kNarrowColumns + 4];
+// shared memory: a lane's columns of them would take a third of its registers.
+template<int SIZE, bool HALVES, int ITEMS>
+__global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm_narrow_kernel(const layer_norm_params p) {
+    constexpr int kColumns = ITEMS * 32 * 4 + 4;
+    __shared__ __align__(16) float parameters[2][kColumns];
     const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    int col[kNarrowItems];
+    int col[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kNarrowItems; ++i) col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
+    for (int i = 0; i < ITEMS; ++i) col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
     const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
     std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
-    raw_quad<SIZE> raw[kNarrowItems];
+    raw_quad<SIZE> raw[ITEMS];
     if (row < p.rows) load_quads(p.x.base + row * p.x.pitch, col, p.columns, p.per_access, raw);
-    for (int c = threadIdx.x; c < kNarrowColumns + 4; c += kNarrowThreads) {
+    for (int c = threadIdx.x; c < kColumns; c += kNarrowThreads) {
         parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
         parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
     }
     __syncthreads();
     for (; row - group < p.rows; row += step) {
-        float v[kNarrowItems][4], sum[1] = {0.0f};
+        float v[ITEMS][4], sum[1] = {0.0f};
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             raw[i].template widen<HALVES>(half, v[i]);
             sum[0] += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
         }
@@ -42,7 +46,7 @@ __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narr
         const float mean = sum[0] / count; // a division: exact for rows of one value
         sum[0] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[i][k] -= mean;
             if (col[i] + 4 > p.columns) {
@@ -58,14 +62,14 @@ __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocks) layer_norm_narr
         if (row >= p.rows) continue;
         if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
-        for (int i = 0; i < kNarrowItems; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
+        for (int i = 0; i < ITEMS; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
             const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
             v[i][0] = fmaf(v[i][0] * rstd, g.x, b.x);
             v[i][1] = fmaf(v[i][1] * rstd, g.y, b.y);
             v[i][2] = fmaf(v[i][2] * rstd, g.z, b.z);
             v[i][3] = fmaf(v[i][3] * rstd, g.w, b.w);
         }
-        activate_as<KIND>(v);
+        activate(p.epilogue, v);
         drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
         store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
     }
@@ -402,16 +406,30 @@ cb200_status launch_wide_forward(const layer_norm_params &p, const wide_shape &s
     return CB200_STATUS_SUCCESS;
 }
 
-template<int SIZE, bool HALVES, int KIND>
+template<int SIZE, bool HALVES, int ITEMS>
+cb200_status launch_narrow(const layer_norm_params &p, cudaStream_t stream) {
+    const std::int64_t per_block = kNarrowThreads / p.lanes, blocks = (p.rows + per_block - 1) / per_block;
+    layer_norm_narrow_kernel<SIZE, HALVES, ITEMS><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * narrow_blocks(ITEMS))), kNarrowThreads, 0, stream>>>(p);
+    count_launch();
+    CB200_CUDA_OK(cudaGetLastError());
+    return CB200_STATUS_SUCCESS;
+}
+
+template<int SIZE, bool HALVES>
 cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream) {
     if (p.columns <= kNarrowColumns) {
-        const std::int64_t per_block = kNarrowThreads / p.lanes, blocks = (p.rows + per_block - 1) / per_block;
-        layer_norm_narrow_kernel<SIZE, HALVES, KIND><<<static_cast<unsigned>(std::min<std::int64_t>(blocks, 148 * kNarrowBlocks)), kNarrowThreads, 0, stream>>>(p);
-        count_launch();
-        CB200_CUDA_OK(cudaGetLastError());
-        return CB200_STATUS_SUCCESS;
+        const narrow_shape narrow = narrow_shape_of(p.columns, kNarrowItems, 5);
+        p.lanes = narrow.lanes;
+        switch (narrow.items) {
+        case 2: return launch_narrow<SIZE, HALVES, 2>(p, stream);
+        case 3: return launch_narrow<SIZE, HALVES, 3>(p, stream);
+        case 4: return launch_narrow<SIZE, HALVES, 4>(p, stream);
+        case 6: return launch_narrow<SIZE, HALVES, 6>(p, stream);
+        default: return launch_narrow<SIZE, HALVES, 8>(p, stream);
+        }
     }
-    // quads of a thread: all but its last lie in the row, with blocks that are a multiple of 32 threads, from 64, 376, 937 and 2,520 quads on
+    // quads of a thread: all but its last lie in the row, with blocks that are a multiple of 32 threads, from 64 quads on with two,
+    // 376 with four, 937 with six and 2,520 with nine
     if (p.columns <= 2048) return launch_rows<SIZE, HALVES, 2>(p, device, stream);
     if (p.columns <= 4 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 4>(p, device, stream);
     if (p.columns <= 6 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 6>(p, device, stream);
@@ -438,9 +456,7 @@ extern "C" cb200_status cb200_layer_norm_forward(const cb200_layer_norm *d, void
     CB200_CUDA_OK(scope.status);
     if (p.rows == 0) return CB200_STATUS_SUCCESS;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return with_epilogue(p.epilogue, [&](auto kind) {
-        if (p.x.dtype == CB200_DTYPE_F16) return launch_forward<2, true, kind()>(p, d->device, s);
-        if (p.x.dtype == CB200_DTYPE_BF16) return p.y.dtype == CB200_DTYPE_F16 ? launch_forward<2, true, kind()>(p, d->device, s) : launch_forward<2, false, kind()>(p, d->device, s);
-        return p.y.dtype == CB200_DTYPE_F16 ? launch_forward<4, true, kind()>(p, d->device, s) : launch_forward<4, false, kind()>(p, d->device, s);
-    });
+    const bool halves = p.x.dtype == CB200_DTYPE_F16 || p.y.dtype == CB200_DTYPE_F16;
+    if (element_bytes(p.x.dtype) == 4) return halves ? launch_forward<4, true>(p, d->device, s) : launch_forward<4, false>(p, d->device, s);
+    return halves ? launch_forward<2, true>(p, d->device, s) : launch_forward<2, false>(p, d->device, s);
 }
