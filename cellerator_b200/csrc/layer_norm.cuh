@@ -186,11 +186,25 @@ __device__ __forceinline__ float tanh_gate(float z, float zz) {
     return fast_reciprocal(1.0f + fast_exp2(z * fmaf(-0.10294324f, zz, -2.3022082f)));
 }
 
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun (C. Hastings, 1955): off by 0.75e-7 at most, 2e-7 with
+// fp32's roundings, and smoothly 0 and 1 far out.  erff, whose branches a warp takes both, made the forward pass of 48 million
+// values with dropout 112 us.  tail: e^(-z z / 2), which the slope needs as well.
+__device__ __forceinline__ float normal_integral(float z, float &tail) {
+    const float t = fast_reciprocal(fmaf(fabsf(z), 0.23164189f, 1.0f)); // 0.3275911 / sqrt 2
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+    tail = fast_exp2(-0.72134752f * z * z);
+    const float outside = poly * tail;
+    return z >= 0.0f ? 1.0f - outside : outside;
+}
+
 // act(z)
 template<int KIND>
 __device__ __forceinline__ float activation(float z) {
     if constexpr (KIND == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
-    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) {
+        float tail;
+        return z * normal_integral(z, tail);
+    }
     if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return z * tanh_gate(z, fminf(z * z, 1e6f));
     return z;
 }
@@ -199,8 +213,11 @@ __device__ __forceinline__ float activation(float z) {
 template<int KIND>
 __device__ __forceinline__ float through_activation(float dy, float z) {
     if constexpr (KIND == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
-    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF)
-        return dy * fmaf(z, 0.39894228f * fast_exp2(-0.72134752f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) {
+        float tail;
+        const float integral = normal_integral(z, tail);
+        return dy * fmaf(z * 0.39894228f, tail, integral);
+    }
     if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) {
         const float zz = fminf(z * z, 1e6f), gate = tanh_gate(z, zz);
         const float steep = fmaf(-gate, gate, gate); // gate (1 - gate): 0 far from 0, times finite numbers

@@ -61,8 +61,9 @@ def norm_forward(x, gamma, beta, eps, kind, factor):
     that and U of itself; the variance, a sum of squares, by 36 U of itself and twice the mean's error times the differences' mean
     (their exact sum is zero; what is left of the mean's error is squared); its reciprocal root by half that, 2 units for rsqrtf
     and 1 for the sum with eps.  u then is off by rstd 34 U mean|x| + 26 U |u|, z by that times |gamma| and 2 U (|gamma u| + |z|).
-    The activations' slopes are below 1.13.  Their own error: erff 2 units of 1, __expf 2 + 1.2 |t| units of itself where it counts
-    (sigma (1 - sigma) |t| < 0.23), a division of 2 units, four products: less than 20 U |z|."""
+    The activations' slopes are below 1.13.  Their own error: Phi by a polynomial that is 0.75e-7 = 1.3 U off, with a reciprocal, five
+    products and sums and an exponential less than 6 U; the logistic function's exponential 4 U + 2 |t| U of itself where it counts
+    (sigma (1 - sigma) |t| < 0.23), a reciprocal of 2 U, four products: less than 20 U |z|."""
     mean = x.mean(1, keepdim=True)
     centred = x - mean
     rstd = 1 / (centred.square().mean(1, keepdim=True) + eps).sqrt()
