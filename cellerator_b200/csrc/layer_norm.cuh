@@ -1,25 +1,20 @@
-// What the forward and the backward pass of the layer norm share: the checks of a call, how rows are shared out, activations,
-// and sums over a row that lies in one warp's lanes, in one block's threads or in a cluster's.
+// What the forward and the backward pass of the layer norm share: the checks of a call, how narrow rows lie in a warp, activations,
+// and sums over lanes.
 #pragma once
 
 #include "counter_random.cuh"
 #include "row_quads.cuh"
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace cb200 {
 
-// Widths.  Up to 1,024 columns (backward 512) a row belongs to a group of lanes of one warp, wider ones to a block.  Forward, the widest belong to a
-// cluster of eight blocks, each with a slice of the columns; backward, rows that no block holds are taken in two passes.
+// Widths.  Up to 1,024 columns (backward 512) a row belongs to a group of lanes of one warp, wider ones to a block; backward, rows that
+// no block holds are taken in two passes.
 constexpr int kBlockColumns = 4608; // of a row that one block holds, backward
 constexpr std::int64_t kMostColumns = 65536;
 constexpr int kNarrowThreads = 256;
-// Most threads of a block of a wide row, by the quads of a thread: eight blocks hold 36,864 columns with two, all 65,536 with four.
-constexpr int wide_threads(int quads_per_thread) { return quads_per_thread == 2 ? 576 : 512; }
-constexpr int kMostWarps = 18;
-constexpr int kMostCluster = 8;
 
 struct layer_norm_params {
     row_matrix x, y, dy, dx;
@@ -30,90 +25,16 @@ struct layer_norm_params {
     int columns;
     int per_access;        // columns that a load or store of every one of the matrices can take
     int lanes;             // narrow: lanes of a row, a power of two
-    int slice_quads;       // wide: quads of a block's slice
-    int cluster;           // wide: blocks of a row
     int epilogue;
     float epsilon;
     dropout_args drop;
 };
-
-// How a wide row is cut: quads per thread, blocks of the cluster, threads of a block.
-struct wide_shape {
-    int quads_per_thread, cluster, threads, slice_quads;
-};
-// As few blocks to a row as hold it (the sums of a row that one block holds need no cluster barrier), with two quads to a thread
-// where eight blocks suffice.
-inline wide_shape wide_shape_of(std::int64_t columns) {
-    wide_shape s{};
-    const int quads = static_cast<int>((columns + 3) / 4);
-    s.quads_per_thread = quads <= 2 * wide_threads(2) * kMostCluster ? 2 : 4;
-    s.cluster = 1;
-    while (s.cluster < kMostCluster && quads > s.quads_per_thread * wide_threads(s.quads_per_thread) * s.cluster) s.cluster *= 2;
-    s.slice_quads = (quads + s.cluster - 1) / s.cluster;
-    s.threads = ((s.slice_quads + s.quads_per_thread - 1) / s.quads_per_thread + 31) / 32 * 32;
-    return s;
-}
 
 // Backward pass of rows that no block holds (layer_norm_columns.cu): parts of the sums of dgamma and dbeta, bytes of the rows' sums,
 // launch.  p.partials (for the parts) and `sums` are the caller's; sums is needed where p.dx is.
 std::int64_t layer_norm_columns_parts(std::int64_t rows, std::int64_t columns);
 std::uint64_t layer_norm_columns_sums_bytes(std::int64_t rows, std::int64_t columns);
 cb200_status launch_layer_norm_columns(const layer_norm_params &p, float *sums, cudaStream_t stream);
-
-// Launches a kernel of a wide row as clusters.
-template<typename K>
-cudaError_t launch_wide(K kernel, const layer_norm_params &p, const wide_shape &shape, unsigned clusters, std::size_t smem, cudaStream_t stream) {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = static_cast<unsigned>(shape.cluster);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(clusters * static_cast<unsigned>(shape.cluster));
-    config.blockDim = dim3(static_cast<unsigned>(shape.threads));
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = shape.cluster > 1 ? 1u : 0u;
-    return cudaLaunchKernelEx(&config, kernel, p);
-}
-
-// Clusters of this shape that the device holds at once, at least one.  Asked for once for each shape, whose shared memory follows
-// from it (the answer is a property of the kernel and the device).
-template<auto kernel>
-unsigned resident_clusters(const wide_shape &shape, std::size_t smem, int device) {
-    constexpr int kDevices = 64;
-    static std::atomic<unsigned> known[kDevices][kMostCluster + 1][kMostWarps + 1];
-    const bool kept = device >= 0 && device < kDevices;
-    if (kept) {
-        const unsigned n = known[device][shape.cluster][shape.threads / 32].load(std::memory_order_relaxed);
-        if (n != 0u) return n;
-    }
-    int found = 0;
-    if (shape.cluster > 1) {
-        cudaLaunchAttribute attribute{};
-        attribute.id = cudaLaunchAttributeClusterDimension;
-        attribute.val.clusterDim.x = static_cast<unsigned>(shape.cluster);
-        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(static_cast<unsigned>(shape.cluster));
-        config.blockDim = dim3(static_cast<unsigned>(shape.threads));
-        config.dynamicSmemBytes = smem;
-        config.attrs = &attribute;
-        config.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess) found = 0;
-    } else {
-        int per_sm = 0, sms = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, shape.threads, smem) == cudaSuccess &&
-            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess)
-            found = per_sm * sms;
-    }
-    if (found < 1) {
-        cudaGetLastError();
-        return 1u;
-    }
-    if (kept) known[device][shape.cluster][shape.threads / 32].store(static_cast<unsigned>(found), std::memory_order_relaxed);
-    return static_cast<unsigned>(found);
-}
 
 // How a narrow row is laid over the lanes of a warp: a power of two of them, with so many quads each that few are left empty (an
 // empty quad costs what a full one does: 8 columns with GELU and dropout took 211 us with four quads to a lane, 112 with two), and
@@ -285,46 +206,6 @@ __device__ __forceinline__ void lane_sums(float (&v)[N], int lanes) {
         for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
     }
 }
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// The columns of a thread of a wide row: quad i of the thread starts at column col[i] (the number of columns where it has none).
-template<int QT>
-__device__ __forceinline__ void wide_columns(const layer_norm_params &p, int rank, int (&col)[QT]) {
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const int quad = i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
-        col[i] = quad < p.slice_quads ? min((rank * p.slice_quads + quad) * 4, p.columns) : p.columns;
-    }
-}
-
-// What the warps of a block, or of a cluster of blocks, tell each other of a step of rows: N numbers a warp.  A warp leaves its
-// numbers with every block, and behind a barrier every warp reads all of them, in the same order.  A cluster works on one step's
-// numbers while the next one's are on their way, so that three sets are in use: what is written for a step was read three steps
-// before, and every thread has passed a barrier since.
-template<int N, bool CLUSTER>
-struct wide_notes {
-    static constexpr int kSets = CLUSTER ? 3 : 2;
-    float note[kSets][(CLUSTER ? kMostCluster : 1) * kMostWarps][N];
-
-    __device__ __forceinline__ void leave(const float (&v)[N], int set, int rank, int cluster) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        float *mine = note[set][rank * warps + warp];
-        if constexpr (CLUSTER) {
-            if (lane < cluster) {
-                std::uint32_t there;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<std::uint32_t>(__cvta_generic_to_shared(mine))), "r"(lane));
-#pragma unroll
-                for (int k = 0; k < N; ++k) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + 4u * k), "f"(v[k]) : "memory");
-            }
-        } else if (lane == 0) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) mine[k] = v[k];
-        }
-    }
-};
-__device__ __forceinline__ int next_set(int set, int sets) { return set + 1 == sets ? 0 : set + 1; }
 
 template<int N>
 __device__ __forceinline__ void warp_sums(float (&v)[N]) {

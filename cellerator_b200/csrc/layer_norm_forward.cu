@@ -4,6 +4,8 @@
 // from it, so that a row far from zero loses nothing.
 #include "layer_norm.cuh"
 
+#include <atomic>
+
 namespace cb200 {
 namespace {
 
@@ -75,11 +77,74 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm
     }
 }
 
-// A block per row, the row in registers, its next row on the way where two fit; gamma and beta stay in shared memory from row to
-// row, as many columns of them as it holds (the rest of beta comes out of L2).  Each warp takes the mean of its columns and the
-// squares of what differs from that; from all warps' numbers come the row's mean and variance,
-//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
-// with one barrier between them.
+// Mean and variance of a row that a block's threads hold, in one walk over the values and with one barrier.  Each thread sums up
+// its columns' distances from a centre of its own, the mean of its first quad, and their squares: the square of how far that is
+// from the mean of all its columns is at most the number of its quads times their variance, so no digits are lost to the difference
+// in the end.  From {sum, squares about its mean} of each thread come those of the warps, and from these
+//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2).
+struct block_statistics {
+    float notes[2][2][32], sizes[32], inverses[32]; // of the warps: of two rows in turn; columns
+
+    // before the first row; own: columns of the thread
+    __device__ __forceinline__ void begin(float own) {
+        float size[1] = {own};
+        warp_sums(size);
+        if ((threadIdx.x & 31) == 0) {
+            sizes[threadIdx.x >> 5] = size[0];
+            inverses[threadIdx.x >> 5] = size[0] > 0.0f ? 1.0f / size[0] : 0.0f;
+        }
+        __syncwarp();
+    }
+    // {mean, 1 / sqrt(var + epsilon)}.  moved, spread: sums of the thread's distances from `centre` and of their squares.
+    __device__ __forceinline__ float2 of_row(int set, float own, float own_inverse, float centre, float moved, float spread, float count, float epsilon) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        float t[1] = {fmaf(own, centre, moved)};
+        const float off = moved * own_inverse; // of the thread's mean from its centre
+        warp_sums(t);
+        if (lane == 0) notes[set][0][warp] = t[0];
+        const float differs = (centre - t[0] * inverses[warp]) + off;
+        t[0] = fmaf(own * differs, differs, fmaf(-moved, off, spread));
+        warp_sums(t);
+        if (lane == 0) notes[set][1][warp] = t[0];
+        __syncthreads();
+        const float of_warp = lane < warps ? notes[set][0][lane] : 0.0f;
+        t[0] = of_warp;
+        warp_sums(t);
+        const float mean = t[0] / count; // a division: exact for rows of one value
+        t[0] = 0.0f;
+        if (lane < warps) {
+            const float from = fmaf(of_warp, inverses[lane], -mean);
+            t[0] = fmaf(sizes[lane] * from, from, notes[set][1][lane]);
+        }
+        warp_sums(t);
+        return make_float2(mean, rsqrtf(fmaf(t[0], 1.0f / count, epsilon)));
+    }
+};
+
+// The sums of a thread's distances from its centre, a quad at a time.
+struct thread_statistics {
+    pair minus, moved, spread;
+    __device__ __forceinline__ explicit thread_statistics(float centre) : minus(-centre), moved(0.0f), spread(0.0f) {}
+    __device__ __forceinline__ void add(const float (&v)[4]) {
+        const pair d = pair(v[0], v[1]) + minus, e = pair(v[2], v[3]) + minus;
+        moved = moved + d;
+        spread = fma(d, d, spread);
+        moved = moved + e;
+        spread = fma(e, e, spread);
+    }
+};
+// Columns from n on, of a quad that starts at column `at`, count as the centre.
+__device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float centre) {
+    if (at + 4 <= n) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (at + k >= n) v[k] = centre;
+}
+
+// A block per row, the row in registers, its next row on the way where two fit and asked for in L2 where not; gamma and beta stay in
+// shared memory from row to row, as many columns of them as it holds (the rest of beta comes out of L2).
+// 4,099 x 33,538 bf16: 176 us, bound by the instructions of 30 warps an SM (26 a value; 41 with branches for each quad: 277 us); a cluster
+// of eight blocks per row, whose threads kept gamma and beta of their columns, took 373 us, waiting for its barriers.
 constexpr int kRowThreads = 1024;
 constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
 constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
@@ -89,8 +154,8 @@ template<int SIZE, bool HALVES, int QT>
 __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const layer_norm_params p, int beta_quads) {
     constexpr bool kAhead = QT * SIZE <= 16; // registers for two rows
     extern __shared__ __align__(16) float parameters[]; // gamma, then beta of each thread's first beta_quads quads
-    __shared__ float notes[2][2][32], sizes[32], inverses[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = p.columns, width = static_cast<int>(blockDim.x) * 4;
+    __shared__ block_statistics statistics;
+    const int n = p.columns, width = static_cast<int>(blockDim.x) * 4;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
     const int padded = (n + 3) & ~3;
@@ -107,13 +172,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
         parameters[c] = p.gamma != nullptr && c < n ? __ldg(p.gamma + c) : 1.0f;
         if (c < beta_quads * width) parameters[padded + 4 + c] = p.beta != nullptr && c < n ? __ldg(p.beta + c) : 0.0f;
     }
-    const int left = n - (QT - 1) * width - warp * 128; // columns of the warp's last quads
-    const float size = static_cast<float>((QT - 1) * 128 + min(max(left, 0), 128)), inverse_size = 1.0f / size, count = static_cast<float>(n), inverse = 1.0f / count;
-    if (lane == 0) {
-        sizes[warp] = size;
-        inverses[warp] = inverse_size;
-    }
     const float own_columns = static_cast<float>(4 * (QT - 1) + min(max(n - col[QT - 1], 0), 4)), own_inverse = 1.0f / own_columns;
+    statistics.begin(own_columns);
     int set = 0;
     const std::int64_t ahead = kAhead ? 2 : 1; // rows, of this block's, that L2 is asked for in advance
     for (; row < p.rows; row += gridDim.x, set ^= 1) {
@@ -122,56 +182,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
         if constexpr (kAhead) {
             if (row + gridDim.x < p.rows) load_quads<QT - 1>(p.x.base + (row + gridDim.x) * p.x.pitch, col, n, p.per_access, next);
         }
-        // this thread's columns about the mean of its first quad, in one walk: the square of how far that is from the mean of all of
-        // them is at most (QT - 1) times their variance, so no digits are lost to the difference at the end
-        float centre, moved, spread;
-        {
-            float v[4];
-            now[0].template widen<HALVES>(half, v);
-            centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
-            const pair minus(-centre);
-            pair s(0.0f), q(0.0f);
+        float v[4];
+        now[0].template widen<HALVES>(half, v);
+        const float centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
+        thread_statistics sums(centre);
 #pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                now[i].template widen<HALVES>(half, v);
-                if (i == QT - 1 && col[i] + 4 > n) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (col[i] + k >= n) v[k] = centre;
-                }
-                const pair d = pair(v[0], v[1]) + minus, e = pair(v[2], v[3]) + minus;
-                s = s + d;
-                q = fma(d, d, q);
-                s = s + e;
-                q = fma(e, e, q);
-            }
-            moved = s.sum();
-            spread = q.sum();
+        for (int i = 0; i < QT; ++i) {
+            now[i].template widen<HALVES>(half, v);
+            if (i == QT - 1) cut_off(v, col[i], n, centre);
+            sums.add(v);
         }
-        // {sum, sum of squares about the warp's mean} of the warp
-        float t[1] = {fmaf(own_columns, centre, moved)};
-        const float own_off = moved * own_inverse; // of the thread's mean from its centre
-        warp_sums(t);
-        if (lane == 0) notes[set][0][warp] = t[0];
-        {
-            const float differs = (centre - t[0] * inverse_size) + own_off;
-            t[0] = fmaf(own_columns * differs, differs, fmaf(-moved, own_off, spread));
-        }
-        warp_sums(t);
-        if (lane == 0) notes[set][1][warp] = t[0];
-        __syncthreads();
-        const float of_warp = lane < warps ? notes[set][0][lane] : 0.0f;
-        t[0] = of_warp;
-        warp_sums(t);
-        const float mean = t[0] / count; // exact for rows of one value
-        t[0] = 0.0f;
-        if (lane < warps) {
-            const float differs = fmaf(of_warp, inverses[lane], -mean);
-            t[0] = fmaf(sizes[lane] * differs, differs, notes[set][1][lane]);
-        }
-        warp_sums(t);
-        const float rstd = rsqrtf(fmaf(t[0], inverse, p.epsilon));
-        if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+        const float2 s = statistics.of_row(set, own_columns, own_inverse, centre, sums.moved.sum(), sums.spread.sum(), static_cast<float>(n), p.epsilon);
+        const float mean = s.x, rstd = s.y;
+        if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = s;
         // a few quads at a time: what is computed takes twice the registers of what was loaded
         constexpr int B = QT % 3 == 0 ? 3 : 2;
         unsigned char *y = p.y.base + row * p.y.pitch;
@@ -228,182 +251,68 @@ cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t st
     return CB200_STATUS_SUCCESS;
 }
 
-// Rows of a step of a wide kernel.
-template<int SIZE, int QT>
-constexpr int kWideRows = (QT == 2 ? 8 : 4) / SIZE;
+// Rows that do not fit the registers: a block walks along its row twice, the second time out of L2.  40,000 columns, 48 million values:
+// fp32 XX us, bf16 XX us, bound by what L2 delivers (the row twice, gamma and beta); clusters of eight blocks that held a row 183 and 122.
+constexpr int kLongThreads = 512, kLongQuads = 4; // quads that a thread has in flight
 
-// A block, or a cluster of blocks that take a slice of the columns each, works on R rows at a time.  Each warp takes the mean of
-// its columns and the squares of what differs from that; from all warps' numbers come the row's mean and variance,
-//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
-// with one exchange between them.  In a cluster the exchange of one step of rows goes round while the step before is written
-// and the one behind it is summed.
-template<int SIZE, bool HALVES, int QT, bool CLUSTER>
-__global__ void __launch_bounds__(wide_threads(QT)) layer_norm_wide_kernel(const layer_norm_params p) {
-    constexpr int R = kWideRows<SIZE, QT>;
-    __shared__ wide_notes<2 * R, CLUSTER> notes;
-    __shared__ float sizes[(CLUSTER ? kMostCluster : 1) * kMostWarps]; // columns of each warp
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, all_warps = p.cluster * warps;
-    const int rank = CLUSTER ? static_cast<int>(blockIdx.x) % p.cluster : 0;
-    const std::int64_t first = (CLUSTER ? blockIdx.x / p.cluster : blockIdx.x) * static_cast<std::int64_t>(R);
-    const std::int64_t stride = (CLUSTER ? gridDim.x / p.cluster : gridDim.x) * static_cast<std::int64_t>(R);
+template<int SIZE, bool HALVES>
+__global__ void __launch_bounds__(kLongThreads, 2) layer_norm_long_kernel(const layer_norm_params p) {
+    __shared__ block_statistics statistics;
+    constexpr int kStep = kLongThreads * 4;
+    const int n = p.columns, first = static_cast<int>(threadIdx.x) * 4;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
-    float gamma[QT][4], beta[QT][4];
-    int col[QT];
-    wide_columns<QT>(p, rank, col);
+    float own = 0.0f;
+    for (int at = first; at < n; at += kStep) own += static_cast<float>(min(4, n - at));
+    const float own_inverse = 1.0f / own; // a thread has columns: there are more than 2,048 of them
+    statistics.begin(own);
+    int set = 0;
+    for (std::int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, set ^= 1) {
+        const unsigned char *x = p.x.base + row * p.x.pitch;
+        unsigned char *y = p.y.base + row * p.y.pitch;
+        float centre = 0.0f;
+        thread_statistics sums(0.0f);
+        for (int at = first; at < n; at += kLongQuads * kStep) {
+            raw_quad<SIZE> raw[kLongQuads];
+            int col[kLongQuads];
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        load_parameters(p.gamma, col[i], p.columns, 1.0f, gamma[i]);
-        load_parameters(p.beta, col[i], p.columns, 0.0f, beta[i]);
-    }
-    const auto columns_of = [&](int w) { // of warp w of the block with this rank
-        return [&, w](int of_rank) {
-            int n = 0;
-            for (int i = 0; i < QT; ++i) {
-                const int begin = i * static_cast<int>(blockDim.x) + w * 32, end = min(begin + 32, p.slice_quads);
-                if (begin < end) n += max(0, min((of_rank * p.slice_quads + end) * 4, p.columns) - min((of_rank * p.slice_quads + begin) * 4, p.columns));
-            }
-            return n;
-        };
-    };
-    for (int i = threadIdx.x; i < all_warps; i += blockDim.x) sizes[i] = static_cast<float>(columns_of(i % warps)(i / warps));
-    const float size = static_cast<float>(columns_of(warp)(rank)), inverse_size = size > 0.0f ? 1.0f / size : 0.0f;
-    const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
-
-    raw_quad<SIZE> now[R][QT], next[R][QT], before[R][QT];
-    const auto fetch = [&](raw_quad<SIZE> (&raw)[R][QT], std::int64_t at) {
+            for (int i = 0; i < kLongQuads; ++i) col[i] = min(at + i * kStep, (n + 3) & ~3);
+            load_quads(x, col, n, p.per_access, raw);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (at + r < p.rows) load_quads(p.x.base + (at + r) * p.x.pitch, col, p.columns, p.per_access, raw[r]);
-        }
-    };
-    // {sum, squares of what differs from the warp's mean} of each row
-    const auto summed = [&](float (&v)[2 * R]) {
-        float t[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            t[r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                float x[4];
-                now[r][i].template widen<HALVES>(half, x);
-                t[r] += (x[0] + x[1]) + (x[2] + x[3]);
-            }
-        }
-        warp_sums<R>(t);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            v[r] = t[r];
-            const float mean = t[r] * inverse_size;
-            t[r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                float x[4];
-                now[r][i].template widen<HALVES>(half, x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] -= mean;
-                if (col[i] + 4 > p.columns) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (col[i] + k >= p.columns) x[k] = 0.0f;
+            for (int i = 0; i < kLongQuads; ++i) {
+                float v[4];
+                raw[i].template widen<HALVES>(half, v);
+                if (i == 0 && at == first) {
+                    centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
+                    sums.minus = pair(-centre);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) t[r] = fmaf(x[k], x[k], t[r]);
+                cut_off(v, col[i], n, centre);
+                sums.add(v);
             }
         }
-        warp_sums<R>(t);
+        const float2 s = statistics.of_row(set, own, own_inverse, centre, sums.moved.sum(), sums.spread.sum(), static_cast<float>(n), p.epsilon);
+        if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = s;
+        for (int at = first; at < n; at += kLongQuads * kStep) {
+            raw_quad<SIZE> raw[kLongQuads];
+            int col[kLongQuads];
+            float v[kLongQuads][4];
 #pragma unroll
-        for (int r = 0; r < R; ++r) v[R + r] = t[r];
-    };
-    const auto finish = [&](const raw_quad<SIZE> (&raw)[R][QT], std::int64_t at, int set) {
-        float mean[R], var[R];
+            for (int i = 0; i < kLongQuads; ++i) col[i] = min(at + i * kStep, (n + 3) & ~3);
+            load_quads(x, col, n, p.per_access, raw);
 #pragma unroll
-        for (int r = 0; r < R; ++r) mean[r] = var[r] = 0.0f;
-        for (int w = lane; w < all_warps; w += 32) {
+            for (int i = 0; i < kLongQuads; ++i) {
+                float g[4], b[4];
+                load_parameters(p.gamma, col[i], n, 1.0f, g);
+                load_parameters(p.beta, col[i], n, 0.0f, b);
+                raw[i].template widen<HALVES>(half, v[i]);
 #pragma unroll
-            for (int r = 0; r < R; ++r) mean[r] += notes.note[set][w][r];
-        }
-        warp_sums<R>(mean);
-#pragma unroll
-        for (int r = 0; r < R; ++r) mean[r] /= count; // exact for rows of one value
-        for (int w = lane; w < all_warps; w += 32) {
-            const float n = sizes[w], over = n > 0.0f ? 1.0f / n : 0.0f;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float off = fmaf(notes.note[set][w][r], over, -mean[r]);
-                var[r] += fmaf(n * off, off, notes.note[set][w][R + r]);
-            }
-        }
-        warp_sums<R>(var);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const std::int64_t row = at + r;
-            if (row >= p.rows) break;
-            const float rstd = rsqrtf(var[r] * inverse + p.epsilon);
-            if (p.stats != nullptr && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean[r], rstd);
-            float v[QT][4];
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                raw[r][i].template widen<HALVES>(half, v[i]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - mean[r]) * rstd, gamma[i][k], beta[i][k]);
+                for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - s.x) * s.y, g[k], b[k]);
             }
             activate(p.epilogue, v);
             drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
-            store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
-        }
-    };
-
-    fetch(now, first);
-    int set = 0;
-    if constexpr (CLUSTER) {
-        cluster_arrive(); // every block of the cluster has begun
-        std::int64_t row = first;
-        for (; row < p.rows; row += stride) {
-            float v[2 * R];
-            summed(v);
-            cluster_wait();
-            notes.leave(v, set, rank, p.cluster);
-            cluster_arrive();
-            fetch(next, row + stride);
-            if (row != first) finish(before, row - stride, set == 0 ? 2 : set - 1);
-            set = next_set(set, 3);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-#pragma unroll
-                for (int i = 0; i < QT; ++i) {
-                    before[r][i] = now[r][i];
-                    now[r][i] = next[r][i];
-                }
-            }
-        }
-        cluster_wait();
-        if (row != first) finish(before, row - stride, set == 0 ? 2 : set - 1);
-    } else {
-        for (std::int64_t row = first; row < p.rows; row += stride, set ^= 1) {
-            float v[2 * R];
-            summed(v);
-            notes.leave(v, set, rank, p.cluster);
-            fetch(next, row + stride);
-            __syncthreads();
-            finish(now, row, set);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-#pragma unroll
-                for (int i = 0; i < QT; ++i) now[r][i] = next[r][i];
-            }
+            store_quads<HALVES>(y, col, n, p.per_access, p.y.dtype, v);
         }
     }
-}
-
-template<int SIZE, bool HALVES, int QT, bool CLUSTER>
-cb200_status launch_wide_forward(const layer_norm_params &p, const wide_shape &shape, int device, cudaStream_t stream) {
-    constexpr auto kernel = layer_norm_wide_kernel<SIZE, HALVES, QT, CLUSTER>;
-    constexpr int step = kWideRows<SIZE, QT>;
-    const std::int64_t clusters = std::min<std::int64_t>((p.rows + step - 1) / step, resident_clusters<kernel>(shape, 0, device));
-    CB200_CUDA_OK(launch_wide(kernel, p, shape, static_cast<unsigned>(clusters), 0, stream));
-    count_launch();
-    return CB200_STATUS_SUCCESS;
 }
 
 template<int SIZE, bool HALVES, int ITEMS>
@@ -434,10 +343,10 @@ cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream
     if (p.columns <= 4 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 4>(p, device, stream);
     if (p.columns <= 6 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 6>(p, device, stream);
     if (p.columns <= kRowColumns) return launch_rows<SIZE, HALVES, 9>(p, device, stream);
-    const wide_shape shape = wide_shape_of(p.columns);
-    p.cluster = shape.cluster;
-    p.slice_quads = shape.slice_quads;
-    return launch_wide_forward<SIZE, HALVES, 4, true>(p, shape, device, stream);
+    layer_norm_long_kernel<SIZE, HALVES><<<static_cast<unsigned>(std::min<std::int64_t>(p.rows, 148 * 2)), kLongThreads, 0, stream>>>(p);
+    count_launch();
+    CB200_CUDA_OK(cudaGetLastError());
+    return CB200_STATUS_SUCCESS;
 }
 
 } // namespace

@@ -5,6 +5,7 @@ libcellerator_b200.so through `capi`.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 from dataclasses import dataclass, field
 
@@ -522,6 +523,20 @@ def _generator(probability: float, seed: int, sequence: int, first_row: int, dev
     return probability, seed, sequence, device_sequence.data_ptr(), first_row
 
 
+def _result_like(x: torch.Tensor, given: torch.Tensor | None, dtype: torch.dtype | None, name: str):
+    """(matrix, type code, leading dimension) of a result: the given one, which is checked, or a new one of x's shape."""
+    if given is None:
+        given = torch.empty_like(x) if dtype is None or dtype is x.dtype else torch.empty_like(x, dtype=dtype)
+        code = _TORCH_ROWS.get(given.dtype)
+        if code is None:
+            raise ValueError(f"{name}_dtype must be float32, bfloat16 or float16")
+        return given, code, given.stride(0)
+    if dtype is not None and given.dtype is not dtype:
+        raise ValueError(f"{name} has another type than {name}_dtype")
+    code, _, ld = _rows_of(given, name, x.shape)
+    return given, code, ld
+
+
 def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *, first_row: int = 0,
             device_sequence: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """x / (1 - probability) where the counter-based generator keeps the value, else 0 (cb200_dropout_rows).
@@ -530,9 +545,7 @@ def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *
     call on the gradient, and a shard passes the number of its first row.  device_sequence: one int64 on the device that is
     added to sequence when the kernel runs.  out may be x."""
     code, shape, ld = _rows_of(x, "x")
-    if out is None:
-        out = torch.empty_like(x)
-    out_code, _, out_ld = _rows_of(out, "out", shape)
+    out, out_code, out_ld = _result_like(x, out, None, "out")
     generator = _generator(probability, seed, sequence, first_row, device_sequence)
     index = x.get_device()
     _together(index, out, device_sequence)
@@ -543,15 +556,6 @@ def dropout(x: torch.Tensor, probability: float, seed: int, sequence: int = 0, *
 
 def _epilogue_of(epilogue) -> int:
     return capi.EPILOGUE[epilogue] if isinstance(epilogue, str) else int(epilogue)
-
-
-def _rows_like(x: torch.Tensor, given: torch.Tensor | None, dtype: torch.dtype | None, name: str) -> torch.Tensor:
-    """The matrix of a result: the given one, or a new one of x's shape."""
-    if given is None:
-        return torch.empty_like(x) if dtype is None or dtype is x.dtype else torch.empty_like(x, dtype=dtype)
-    if dtype is not None and given.dtype is not dtype:
-        raise ValueError(f"{name} has another type than {name}_dtype")
-    return given
 
 
 def _stats_of(stats: torch.Tensor, rows: int) -> int:
@@ -571,8 +575,7 @@ def layer_norm(x: torch.Tensor, gamma: torch.Tensor | None = None, beta: torch.T
     dropout is a probability; seed, sequence, first_row and device_sequence are those of ops.dropout."""
     code, shape, ld = _rows_of(x, "x")
     rows, columns = shape
-    out = _rows_like(x, out, out_dtype, "out")
-    out_code, _, out_ld = _rows_of(out, "out", shape)
+    out, out_code, out_ld = _result_like(x, out, out_dtype, "out")
     gamma_ptr, beta_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns)
     stats_ptr = 0 if stats is None else _stats_of(stats, rows)
     generator = _generator(dropout, seed, sequence, first_row, device_sequence)
@@ -597,8 +600,7 @@ def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, 
     code, shape, ld = _rows_of(x, "x")
     rows, columns = shape
     dy_code, _, dy_ld = _rows_of(dy, "dy", shape)
-    dx = _rows_like(x, dx, dx_dtype, "dx")
-    dx_code, _, dx_ld = _rows_of(dx, "dx", shape)
+    dx, dx_code, dx_ld = _result_like(x, dx, dx_dtype, "dx")
     gamma_ptr, beta_ptr, stats_ptr = _vector(gamma, "gamma", columns), _vector(beta, "beta", columns), _stats_of(stats, rows)
     if dgamma is None and gamma is not None:
         dgamma = torch.empty_like(gamma)
@@ -620,6 +622,7 @@ def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, 
     return dx, dgamma, dbeta
 
 
+@functools.lru_cache(maxsize=256)
 def layer_norm_backward_workspace(rows: int, columns: int) -> int:
     """Bytes that layer_norm_backward needs for the sums of dgamma and dbeta."""
     need = C.c_uint64()

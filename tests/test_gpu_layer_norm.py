@@ -9,9 +9,11 @@ from row_operators import assert_within, keep, matrix, norm_backward, norm_forwa
 pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
-# one value; less than a quad; a lane; several lanes, with and without a last piece of a quad; the widest row of a warp and the
-# first of a block; several warps; the first of a cluster of 2, of 4, of 8; the gene set; the first of four quads to a thread; the widest
-WIDTHS = [1, 2, 3, 4, 7, 16, 32, 50, 64, 100, 128, 255, 512, 513, 516, 1237, 4608, 4609, 9300, 18_433, 33_538, 36_864, 36_868, 65_536]
+# one value; less than a quad; a lane; several lanes, with and without a last piece of a quad; either side of where a warp's rows end,
+# backward and forward; of two and four quads to a thread, of a block's rows backward, of four, six and nine quads; the gene set; either
+# side of what the registers hold; the widest
+WIDTHS = [1, 2, 3, 4, 7, 16, 32, 50, 64, 100, 128, 255, 512, 513, 700, 1024, 1025, 1237, 2048, 2049, 4608, 4609, 16_384, 16_386, 24_577, 33_538, 36_864,
+          36_868, 65_536]
 
 
 def rows_for(cols):
@@ -282,7 +284,7 @@ def test_parts_of_many_rows(cuda_device, rows, cols, dtype):
 
 def test_graph_replay_on_another_stream(cuda_device):
     """Forward and backward captured together, eager calls in between; new inputs and a new mask at each replay."""
-    for cols in (48, 5000):
+    for cols in (48, 2000, 5000, 40_000):
         x, dy = matrix(200, cols, torch.float32, cuda_device, 103), matrix(200, cols, torch.float32, cuda_device, 104)
         gamma, beta = parameters(cols, cuda_device, 105)
         number = torch.zeros(1, dtype=torch.int64, device=cuda_device)
