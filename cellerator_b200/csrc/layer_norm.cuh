@@ -88,6 +88,16 @@ __device__ __forceinline__ void load_parameters(const float *v, int col, int n, 
     for (int k = 0; k < 4; ++k) out[k] = v != nullptr && col + k < n ? __ldg(v + col + k) : otherwise;
 }
 
+// The same where the vector is known to be there, in one load where `vectors` says that it lies on a 16-byte boundary and the quad
+// lies in it.
+__device__ __forceinline__ float4 load_parameter_quad(const float *v, int col, int n, bool vectors) {
+    if (vectors && col + 4 <= n) return __ldg(reinterpret_cast<const float4 *>(v + col));
+    float w[4];
+    load_parameters(v, col, n, 0.0f, w);
+    return make_float4(w[0], w[1], w[2], w[3]);
+}
+inline __host__ __device__ bool on_16_bytes(const void *p) { return reinterpret_cast<std::uintptr_t>(p) % 16u == 0u; }
+
 // 2^t and 1 / t by the hardware's approximations, within 2 units and 1 unit of the last place; what is too small for a normal number
 // is 0.
 __device__ __forceinline__ float fast_exp2(float t) {

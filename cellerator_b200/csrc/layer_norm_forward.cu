@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) layer_norm_long_kernel(const 
     const int n = p.columns, first = static_cast<int>(threadIdx.x) * 4;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
     const std::uint64_t sequence = sequence_of(p.drop);
+    const bool vectors = on_16_bytes(p.gamma) && on_16_bytes(p.beta);
     float own = 0.0f;
     for (int at = first; at < n; at += kStep) own += static_cast<float>(min(4, n - at));
     const float own_inverse = 1.0f / own; // a thread has columns: there are more than 2,048 of them
@@ -299,14 +300,21 @@ __global__ void __launch_bounds__(kLongThreads, 2) layer_norm_long_kernel(const 
 #pragma unroll
             for (int i = 0; i < kLongQuads; ++i) col[i] = min(at + i * kStep, (n + 3) & ~3);
             load_quads(x, col, n, p.per_access, raw);
+            float4 g[kLongQuads], b[kLongQuads];
 #pragma unroll
             for (int i = 0; i < kLongQuads; ++i) {
-                float g[4], b[4];
-                load_parameters(p.gamma, col[i], n, 1.0f, g);
-                load_parameters(p.beta, col[i], n, 0.0f, b);
-                raw[i].template widen<HALVES>(half, v[i]);
+                g[i] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                b[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (p.gamma != nullptr) g[i] = load_parameter_quad(p.gamma, col[i], n, vectors);
+                if (p.beta != nullptr) b[i] = load_parameter_quad(p.beta, col[i], n, vectors);
+            }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - s.x) * s.y, g[k], b[k]);
+            for (int i = 0; i < kLongQuads; ++i) {
+                raw[i].template widen<HALVES>(half, v[i]);
+                v[i][0] = fmaf((v[i][0] - s.x) * s.y, g[i].x, b[i].x);
+                v[i][1] = fmaf((v[i][1] - s.x) * s.y, g[i].y, b[i].y);
+                v[i][2] = fmaf((v[i][2] - s.x) * s.y, g[i].z, b[i].z);
+                v[i][3] = fmaf((v[i][3] - s.x) * s.y, g[i].w, b[i].w);
             }
             activate(p.epilogue, v);
             drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
