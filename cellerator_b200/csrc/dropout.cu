@@ -103,8 +103,8 @@ extern "C" cb200_status cb200_dropout_rows(const cb200_dropout_matrix *m, void *
     clear_error();
     if (m == nullptr || m->version != CB200_ABI_VERSION || m->size < sizeof(cb200_dropout_matrix))
         return fail(CB200_STATUS_INVALID_ARGUMENT, "bad cb200_dropout_matrix header");
-    if (m->rows < 0 || m->columns < 0 || m->columns > 0x7ffffff0ll || m->rows >= (1ll << 32))
-        return fail(CB200_STATUS_INVALID_SHAPE, "dropout takes fewer than 2^32 rows of fewer than 2^31 columns, got %lld x %lld", (long long)m->rows, (long long)m->columns);
+    if (m->rows < 0 || m->columns < 0 || m->columns > (1ll << 30) || m->rows >= (1ll << 32)) // a place in a row is a 32-bit number of bytes
+        return fail(CB200_STATUS_INVALID_SHAPE, "dropout takes fewer than 2^32 rows of up to 2^30 columns, got %lld x %lld", (long long)m->rows, (long long)m->columns);
     dropout_params p{};
     cb200_status st = row_matrix_of(m->x, m->x_ld, m->x_dtype, m->rows, m->columns, "x", &p.x);
     if (st == CB200_STATUS_SUCCESS) st = row_matrix_of(m->y, m->y_ld, m->y_dtype, m->rows, m->columns, "y", &p.y);

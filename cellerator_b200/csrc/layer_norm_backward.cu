@@ -2,14 +2,13 @@
 //     dz = drop(dy) act'(z),  dbeta = sum over rows of dz,  dgamma = sum over rows of dz u,  h = gamma dz,
 //     dx = rstd (h - mean over columns of h - u mean over columns of (h u)).
 // One pass reads x and dy, keeps a row in registers between its sums and its dx, and adds dz and dz u up per column in the
-// threads that own the columns; a block or cluster leaves its sums in the workspace, and a second launch adds these up in order.
+// threads that own the columns; a block leaves its sums in the workspace, and a second launch adds these up in order.
 #include "dependent_launch.cuh"
 #include "layer_norm.cuh"
 
 namespace cb200 {
 namespace {
 
-// Most blocks of a launch: each leaves 2 x columns sums.
 constexpr int kNarrowItems[] = {2, 4, 3}; // quads of a row that a lane can hold, two by preference (64 columns: 97 us, four 122)
 constexpr std::int64_t kNarrowColumns = 4 * 32 * 4;
 // Blocks that are resident on an SM: with two quads to a lane, which keeps two sums for each of its columns, 24 warps fit.
@@ -251,7 +250,6 @@ std::int64_t block_parts(std::int64_t rows, std::int64_t columns) { return std::
 struct backward_launch {
     layer_norm_params p;
     float *dgamma, *dbeta;
-    int device;
     cudaStream_t stream;
 
     cb200_status finish(std::int64_t parts) const {
@@ -333,7 +331,6 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
     if (p.dx.base != nullptr) p.per_access = columns_per_access(p.dx, p.per_access);
     b.dgamma = d->dgamma;
     b.dbeta = d->dbeta;
-    b.device = d->device;
     b.stream = static_cast<cudaStream_t>(stream);
     device_scope scope(d->device);
     CB200_CUDA_OK(scope.status);

@@ -369,8 +369,10 @@ extern "C" cb200_status cb200_qcsr_adapters(const cb200_adapters *d, void *strea
             return fail(CB200_STATUS_INVALID_ARGUMENT, "adapters: an array is null");
         if (x->bits == 4 && x->packed_row_ptr == nullptr) return fail(CB200_STATUS_INVALID_ARGUMENT, "4-bit codes need packed_row_ptr");
         const std::uintptr_t element = d->weight_dtype == CB200_DTYPE_BF16 ? 2u : 4u;
-        if (reinterpret_cast<std::uintptr_t>(d->down) % element != 0u || reinterpret_cast<std::uintptr_t>(d->up) % element != 0u ||
-            reinterpret_cast<std::uintptr_t>(d->out) % 4u != 0u || reinterpret_cast<std::uintptr_t>(d->adapter) % 4u != 0u)
+        const auto odd = [](const void *a, std::uintptr_t bytes) { return reinterpret_cast<std::uintptr_t>(a) % bytes != 0u; };
+        if (odd(d->down, element) || odd(d->up, element) ||
+            odd(d->out, 4) || odd(d->adapter, 4) || odd(d->scale, 4) || odd(d->bias, 4) || odd(x->row_ptr, 8) || odd(x->packed_row_ptr, 8) ||
+            odd(x->col_idx, 4) || odd(x->scales, 4) || odd(x->offsets, 4))
             return fail(CB200_STATUS_INVALID_ARGUMENT, "adapters: an array is not aligned to its elements");
     }
     device_scope scope(d->device);

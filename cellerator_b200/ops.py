@@ -611,6 +611,8 @@ def layer_norm_backward(x: torch.Tensor, dy: torch.Tensor, stats: torch.Tensor, 
     if workspace is None and rows:
         workspace = stats.new_empty(layer_norm_backward_workspace(rows, columns) // 4)
     if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         workspace_ptr, workspace_bytes = workspace.data_ptr(), workspace.nbytes
     generator = _generator(dropout, seed, sequence, first_row, device_sequence)
     index = x.get_device()

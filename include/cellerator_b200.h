@@ -697,8 +697,8 @@ typedef struct cb200_dropout {
     int64_t first_row;               /* number of row 0; first_row + rows <= 2^32 */
 } cb200_dropout;
 
-/* y = dropout(x) over rows x columns; y may be x (same leading dimension, elements of the same size), else they share no
- * byte.  The gradient is the same call on the gradient of y. */
+/* y = dropout(x) over rows x columns, fewer than 2^32 of up to 2^30; y may be x (same leading dimension, elements of the
+ * same size), else they share no byte.  The gradient is the same call on the gradient of y. */
 typedef struct cb200_dropout_matrix {
     uint32_t version;
     size_t size;
@@ -758,8 +758,9 @@ cb200_status cb200_layer_norm_backward(const cb200_layer_norm *norm, void *strea
  *     out[r] = act(alpha * scale[a] * (deq(X)[r] down[a]) up[a] + beta * out[r] + bias),
  * and without the product where adapter[r] is -1 (or any value outside 0 .. adapters - 1).  beta == 0 never reads out.
  * After a cb200_spmm_run into the same out, beta = 1 adds the adapters to the shared projection, and the epilogue is then
- * this call's; products and sums are fp32.  A gene outside the matrix is left out.  A row's bits follow from its
- * entries, its adapter and the types, not from the rows beside it. */
+ * this call's; products and sums are fp32.  A gene outside the matrix is left out; a row without entries has no product.
+ * A row's bits follow from its entries, its adapter, the types and the alignment of down, not from the rows beside it.
+ * Rows of fewer than 2^31 entries. */
 typedef struct cb200_adapters {
     uint32_t version;
     size_t size;

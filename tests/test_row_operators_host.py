@@ -93,7 +93,7 @@ def test_the_generator_of_the_tests_gives_the_published_words():
 @pytest.mark.parametrize("change,status", [
     (dict(version=1), capi.INVALID_ARGUMENT), (dict(size=8), capi.INVALID_ARGUMENT),
     (dict(rows=-1), capi.INVALID_SHAPE), (dict(columns=-1), capi.INVALID_SHAPE), (dict(rows=2 ** 32 + 1), capi.INVALID_SHAPE),
-    (dict(columns=2 ** 31), capi.INVALID_SHAPE), (dict(x_ld=7), capi.INVALID_SHAPE), (dict(y_ld=7), capi.INVALID_SHAPE),
+    (dict(columns=2 ** 30 + 4, x_ld=2 ** 30 + 4, y_ld=2 ** 30 + 4, rows=1), capi.INVALID_SHAPE), (dict(x_ld=7), capi.INVALID_SHAPE), (dict(y_ld=7), capi.INVALID_SHAPE),
     (dict(x_ld=2 ** 62), capi.INVALID_SHAPE), (dict(x=None), capi.INVALID_ARGUMENT), (dict(y=None), capi.INVALID_ARGUMENT),
     (dict(x=ADDRESS + 2), capi.INVALID_ARGUMENT), (dict(x_dtype=capi.DTYPE_F64), capi.UNSUPPORTED), (dict(y_dtype=capi.DTYPE_U8), capi.UNSUPPORTED),
     (dict(y=ADDRESS + 4), capi.INVALID_ARGUMENT), (dict(y=ADDRESS + 32 * 3), capi.INVALID_ARGUMENT),
@@ -160,6 +160,10 @@ def test_layer_norm_workspace():
     (dict(out_ld=31), {}, capi.INVALID_SHAPE), (dict(row_begin=-1), {}, capi.INVALID_SHAPE), (dict(row_begin=3, row_end=2), {}, capi.INVALID_SHAPE),
     (dict(row_end=5), {}, capi.INVALID_SHAPE), (dict(adapter=None), {}, capi.INVALID_ARGUMENT), (dict(out=None), {}, capi.INVALID_ARGUMENT),
     (dict(down=None), {}, capi.INVALID_ARGUMENT), (dict(up=None), {}, capi.INVALID_ARGUMENT), (dict(up=ADDRESS + 2), {}, capi.INVALID_ARGUMENT),
+    (dict(scale=ADDRESS + 2), {}, capi.INVALID_ARGUMENT), (dict(bias=ADDRESS + 2, epilogue=1), {}, capi.INVALID_ARGUMENT),
+    ({}, dict(row_ptr=ADDRESS + 4), capi.INVALID_ARGUMENT), ({}, dict(bits=4, packed_row_ptr=ADDRESS + 4), capi.INVALID_ARGUMENT),
+    ({}, dict(col_idx=ADDRESS + 2), capi.INVALID_ARGUMENT), ({}, dict(scales=ADDRESS + 1), capi.INVALID_ARGUMENT),
+    ({}, dict(offsets=ADDRESS + 1), capi.INVALID_ARGUMENT),
     ({}, dict(row_ptr=None), capi.INVALID_ARGUMENT), ({}, dict(col_idx=None), capi.INVALID_ARGUMENT), ({}, dict(rows=-1), capi.INVALID_SHAPE),
 ])
 def test_adapters_refuse(change, csr, status):
@@ -215,7 +219,8 @@ def test_python_checks():
                 dict(out=torch.zeros(4, 9)), dict(out=x, out_dtype=torch.float16)):
         with pytest.raises(ValueError):
             ops.layer_norm(x, **bad)
-    for bad in (dict(dy=torch.zeros(5, 8)), dict(stats=torch.zeros(4, 2).half()), dict(dx=x, dx_dtype=torch.float16), dict(dgamma=torch.zeros(9))):
+    for bad in (dict(dy=torch.zeros(5, 8)), dict(stats=torch.zeros(4, 2).half()), dict(dx=x, dx_dtype=torch.float16), dict(dgamma=torch.zeros(9)),
+                dict(workspace=torch.zeros(4096)[::2])):
         with pytest.raises(ValueError):
             ops.layer_norm_backward(x, **{**dict(dy=x, stats=torch.zeros(4, 2)), **bad})
 
