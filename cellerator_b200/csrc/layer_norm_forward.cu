@@ -15,7 +15,9 @@ constexpr std::int64_t kNarrowColumns = 8 * 32 * 4;
 constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
-// shared memory: a lane's columns of them would take a third of its registers.
+// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 71 us, 5.5 TB/s,
+// 84 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
+// once).  GELU and dropout are bound by instructions: 48 million values 93 us.
 template<int SIZE, bool HALVES, int ITEMS>
 __global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm_narrow_kernel(const layer_norm_params p) {
     constexpr int kColumns = ITEMS * 32 * 4 + 4;
@@ -143,8 +145,11 @@ __device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float cent
 
 // A block per row, the row in registers, its next row on the way where two fit and asked for in L2 where not; gamma and beta stay in
 // shared memory from row to row, as many columns of them as it holds (the rest of beta comes out of L2).
-// 4,099 x 33,538 bf16: 176 us, bound by the instructions of 30 warps an SM (26 a value; 41 with branches for each quad: 277 us); a cluster
-// of eight blocks per row, whose threads kept gamma and beta of their columns, took 373 us, waiting for its barriers.
+// 4,099 x 33,538 bf16: 178 us, 47 % of a copy.  Half of the issue slots are taken (25 instructions a value; 41 with branches for each quad,
+// 277 us), and 30 warps, all at the same step of the same row, do not fill the others.  Measured against it: a cluster of eight blocks
+// per row, whose threads kept gamma and beta of their columns, 373 us, waiting for its barriers; 512 threads with twice the quads 260;
+// the next row's quads loaded as soon as these are stored 180; one quad at a time, or two-wide products, 190 (spills); the
+// columns walked twice as below 212.
 constexpr int kRowThreads = 1024;
 constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
 constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
@@ -252,7 +257,8 @@ cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t st
 }
 
 // Rows that do not fit the registers: a block walks along its row twice, the second time out of L2.  40,000 columns, 48 million values:
-// fp32 XX us, bf16 XX us, bound by what L2 delivers (the row twice, gamma and beta); clusters of eight blocks that held a row 183 and 122.
+// fp32 97 us, bf16 68 us, bound by what L2 delivers (the row twice, gamma and beta: 116 and 94 with one column of these to a load);
+// clusters of eight blocks that held a row took 183 and 122.
 constexpr int kLongThreads = 512, kLongQuads = 4; // quads that a thread has in flight
 
 template<int SIZE, bool HALVES>
