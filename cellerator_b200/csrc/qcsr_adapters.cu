@@ -112,11 +112,13 @@ __device__ __forceinline__ void load4(const WT *p, float (&w)[4]) {
 // Lanes past a part's end read its last entry again, and genes outside the matrix row 0 of A: both are staged as gene -1, whose row
 // counts as zeros whatever it holds.  Segments without such entries, nearly all, take the branch that does not look.
 //
-// Bound by what the SMs get out of L2 in pieces of 32 bytes at random places, near 12 TB/s: a row of A, a scale and a zero-point for
-// each entry.  4,099 x 33,538, 8 bits, rank 16 bf16: 78 us; 50,000 x 4,000, 4 bits, rank 32: 298 us (before loads lost their branches
-// 104 and 437).  Measured against it: the rows of one adapter together and slices of its A in shared memory 112 and 430 us; a third
-// stage of loads under way 84; rows of A kept in L1 79 and 298; scales and zero-points side by side, laid so in a launch before, 77 and
-// 305; parts of 256 entries 86 and 369; four blocks an SM by launch bounds 93.
+// 4,099 x 33,538, 8 bits, rank 16 bf16: 75 us, bound by what the SMs get out of L2 in pieces of 32 bytes at random places (a row of A, a
+// scale and a zero-point for each entry).  50,000 x 4,000, 4 bits, rank 32: 292 us, bound by L1's wavefronts (72 %, two for an entry) and
+// instructions (62 % of the slots, six for an entry in its share of a warp).  Before loads lost their branches 104 and 437.  Measured
+// against it: scales and zero-points in shared memory, with fewer blocks an SM, 112 and 430 us; a third stage of loads under way 84; rows
+// of A kept in L1 79 and 298; scales and zero-points side by side, laid so in a launch before, 77 and 305; parts of 256 entries 86 and
+// 369; four blocks an SM by launch bounds 93; every part's sum by a butterfly over all columns, and partial segments wholly in the
+// branch that looks, 78 and 298.
 template<int BITS, typename WT, int V>
 __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
     __shared__ __align__(16) int2 staged[kWarps][kSegment];
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
             const int count = min(kSegment, to - at), part_now = part;
             const unsigned char *down = p.down + static_cast<std::int64_t>(row_adapter[r]) * p.cols * row_bytes + (holds ? col : 0) * sizeof(WT);
             float scale[kRuns], offset[kRuns];
-            bool fine = count == kSegment && holds;
+            bool fine = holds;
             unsigned at_gene[kRuns];
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) {
@@ -225,48 +227,70 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
                 fetch();
             }
             const int2 *mine = stage + group;
+            int e = 0;
             if (fine) {
-                const auto add = [&](auto unrolled, int e) {
+                const auto add = [&](auto unrolled, int first) {
                     constexpr int U = decltype(unrolled)::value;
                     slice<WT, V> w[U];
                     float v[U];
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        const int2 entry = mine[e + u * groups];
+                        const int2 entry = mine[first + u * groups];
                         v[u] = __int_as_float(entry.y);
                         w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(entry.x)) * row_bytes);
                     }
 #pragma unroll
                     for (int u = 0; u < U; ++u) w[u].add_to(acc, v[u]);
                 };
-                if (groups == 32) add(std::integral_constant<int, 4>{}, 0); // one entry to a lane
-                else
-                    for (int e = 0; e < kSegment; e += 8 * groups) add(std::integral_constant<int, 8>{}, e);
-            } else {
-                for (int e = 0; e < count; e += 4 * groups) {
-                    slice<WT, V> w[4];
-                    float v[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int2 entry = mine[e + u * groups];
-                        const bool held = entry.x >= 0 && holds;
-                        v[u] = held ? __int_as_float(entry.y) : 0.0f;
-                        w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(max(entry.x, 0))) * row_bytes);
-                        w[u].keep_if(held);
+                if (groups == 32) { // one entry to a lane
+                    if (count == kSegment) {
+                        add(std::integral_constant<int, 4>{}, 0);
+                        e = kSegment;
                     }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) w[u].add_to(acc, v[u]);
+                } else {
+                    for (; e + 8 * groups <= count; e += 8 * groups) add(std::integral_constant<int, 8>{}, e);
                 }
+            }
+            for (; e < count; e += 4 * groups) {
+                slice<WT, V> w[4];
+                float v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int2 entry = mine[e + u * groups];
+                    const bool held = entry.x >= 0 && holds;
+                    v[u] = held ? __int_as_float(entry.y) : 0.0f;
+                    w[u].load(down + static_cast<std::uint64_t>(static_cast<std::uint32_t>(max(entry.x, 0))) * row_bytes);
+                    w[u].keep_if(held);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u].add_to(acc, v[u]);
             }
             __syncwarp();
             if (!ends) continue;
-            for (int off = lanes; off < 32; off <<= 1) {
+            // the classes' sums: in each step a lane gives half of its columns away and keeps the sums of the other half
+            int kept = V, from = 0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
+            for (int step = 0; step < 5; ++step) {
+                const int off = lanes << step;
+                if (off >= 32) break;
+                if ((V >> step) > 1) {
+                    const int w = (V >> step) / 2;
+                    const bool upper = (lane & off) != 0;
+#pragma unroll
+                    for (int i = 0; i < w; ++i) {
+                        const float given = upper ? acc[i] : acc[i + w];
+                        acc[i] = (upper ? acc[i + w] : acc[i]) + __shfl_xor_sync(0xffffffffu, given, off);
+                    }
+                    kept = w;
+                    from += upper ? w : 0;
+                } else {
+                    acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], off);
+                }
             }
-            if (group == 0 && holds) {
+            if (group < V && holds) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) sums[part_now * p.rank + col + i] = acc[i];
+                for (int i = 0; i < V; ++i)
+                    if (i < kept) sums[part_now * p.rank + col + from + i] = acc[i];
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.0f;
