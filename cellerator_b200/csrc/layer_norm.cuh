@@ -110,49 +110,80 @@ __device__ __forceinline__ float fast_reciprocal(float t) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
     return r;
 }
+__device__ __forceinline__ pair fast_exp2(pair t) {
+    float lo, hi;
+    t.get(lo, hi);
+    return pair(fast_exp2(lo), fast_exp2(hi));
+}
+__device__ __forceinline__ pair fast_reciprocal(pair t) {
+    float lo, hi;
+    t.get(lo, hi);
+    return pair(fast_reciprocal(lo), fast_reciprocal(hi));
+}
+// z^2, cut off above 10^6, where the tanh form's factor is 0 or 1 long since
+__device__ __forceinline__ pair square(pair z) {
+    float lo, hi;
+    (z * z).get(lo, hi);
+    return pair(fminf(lo, 1e6f), fminf(hi, 1e6f));
+}
 // The factor of the tanh form of GELU, (1 + tanh(c (z + 0.044715 z^3))) / 2 with c = sqrt(2 / pi): the logistic function of twice that
-// argument, within a few units of the last place of 1.  zz: z^2, which may be cut off above 10^6 (the factor is 0 or 1 long before).
-__device__ __forceinline__ float tanh_gate(float z, float zz) {
+// argument, within a few units of the last place of 1.  zz: square(z).
+__device__ __forceinline__ pair tanh_gate(pair z, pair zz) {
     // -2 c / ln 2 and 0.044715 of it
-    return fast_reciprocal(1.0f + fast_exp2(z * fmaf(-0.10294324f, zz, -2.3022082f)));
+    return fast_reciprocal(fast_exp2(z * fma(pair(-0.10294324f), zz, pair(-2.3022082f))) + pair(1.0f));
 }
 
 // Phi(z) = (1 + erf(z / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun (C. Hastings, 1955): off by 0.75e-7 at most, 2e-7 with
 // fp32's roundings, and smoothly 0 and 1 far out.  erff, whose branches a warp takes both, made the forward pass of 48 million
 // values with dropout 112 us.  tail: e^(-z z / 2), which the slope needs as well.
-__device__ __forceinline__ float normal_integral(float z, float &tail) {
-    const float t = fast_reciprocal(fmaf(fabsf(z), 0.23164189f, 1.0f)); // 0.3275911 / sqrt 2
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-    tail = fast_exp2(-0.72134752f * z * z);
-    const float outside = poly * tail;
-    return z >= 0.0f ? 1.0f - outside : outside;
+__device__ __forceinline__ pair normal_integral(pair z, pair &tail) {
+    float lo, hi;
+    z.get(lo, hi);
+    const pair t = fast_reciprocal(fma(pair(fabsf(lo), fabsf(hi)), pair(0.23164189f), pair(1.0f))); // 0.3275911 / sqrt 2
+    pair poly = fma(t, pair(0.5307027145f), pair(-0.7265760135f));
+    poly = fma(t, poly, pair(0.7107068705f));
+    poly = fma(t, poly, pair(-0.142248368f));
+    poly = t * fma(t, poly, pair(0.127414796f));
+    tail = fast_exp2(z * pair(-0.72134752f) * z);
+    float outside_lo, outside_hi;
+    (poly * tail).get(outside_lo, outside_hi);
+    return pair(lo >= 0.0f ? 1.0f - outside_lo : outside_lo, hi >= 0.0f ? 1.0f - outside_hi : outside_hi);
 }
 
 // act(z)
 template<int KIND>
-__device__ __forceinline__ float activation(float z) {
-    if constexpr (KIND == CB200_EPILOGUE_RELU) return z < 0.0f ? 0.0f : z; // NaN stays
-    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) {
-        float tail;
-        return z * normal_integral(z, tail);
+__device__ __forceinline__ pair activation(pair z) {
+    if constexpr (KIND == CB200_EPILOGUE_RELU) {
+        float lo, hi;
+        z.get(lo, hi);
+        return pair(lo < 0.0f ? 0.0f : lo, hi < 0.0f ? 0.0f : hi); // NaN stays
     }
-    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return z * tanh_gate(z, fminf(z * z, 1e6f));
+    if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) {
+        pair tail(0.0f);
+        return normal_integral(z, tail) * z;
+    }
+    if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) return tanh_gate(z, square(z)) * z;
     return z;
 }
 
 // dy act'(z); relu's slope is 0 at 0, and lets nothing of dy through there
 template<int KIND>
-__device__ __forceinline__ float through_activation(float dy, float z) {
-    if constexpr (KIND == CB200_EPILOGUE_RELU) return z <= 0.0f ? 0.0f : dy;
+__device__ __forceinline__ pair through_activation(pair dy, pair z) {
+    if constexpr (KIND == CB200_EPILOGUE_RELU) {
+        float lo, hi, dy_lo, dy_hi;
+        z.get(lo, hi);
+        dy.get(dy_lo, dy_hi);
+        return pair(lo <= 0.0f ? 0.0f : dy_lo, hi <= 0.0f ? 0.0f : dy_hi);
+    }
     if constexpr (KIND == CB200_EPILOGUE_GELU_ERF) {
-        float tail;
-        const float integral = normal_integral(z, tail);
-        return dy * fmaf(z * 0.39894228f, tail, integral);
+        pair tail(0.0f);
+        const pair integral = normal_integral(z, tail);
+        return fma(z * pair(0.39894228f), tail, integral) * dy;
     }
     if constexpr (KIND == CB200_EPILOGUE_GELU_TANH) {
-        const float zz = fminf(z * z, 1e6f), gate = tanh_gate(z, zz);
-        const float steep = fmaf(-gate, gate, gate); // gate (1 - gate): 0 far from 0, times finite numbers
-        return dy * fmaf(z * steep, fmaf(0.21406445f, zz, 1.5957691f), gate); // 2 c and 3 times 0.044715 of it
+        const pair zz = square(z), gate = tanh_gate(z, zz);
+        const pair steep = fma(gate, pair(-1.0f), pair(1.0f)) * gate; // 0 far from 0, times finite numbers
+        return fma(z * steep, fma(pair(0.21406445f), zz, pair(1.5957691f)), gate) * dy; // 2 c and 3 times 0.044715 of it
     }
     return dy;
 }
@@ -163,7 +194,7 @@ __device__ __forceinline__ void activate_as(float (&v)[Q][4]) {
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[i][k] = activation<KIND>(v[i][k]);
+        for (int k = 0; k < 4; k += 2) activation<KIND>(pair(v[i][k], v[i][k + 1])).get(v[i][k], v[i][k + 1]);
     }
 }
 template<int Q>
@@ -178,10 +209,8 @@ template<int KIND, int Q>
 __device__ __forceinline__ void through_as(float (&dy)[Q][4], const float (&u)[Q][4], const float4 (&gamma)[Q], const float4 (&beta)[Q]) {
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-        dy[i][0] = through_activation<KIND>(dy[i][0], fmaf(u[i][0], gamma[i].x, beta[i].x));
-        dy[i][1] = through_activation<KIND>(dy[i][1], fmaf(u[i][1], gamma[i].y, beta[i].y));
-        dy[i][2] = through_activation<KIND>(dy[i][2], fmaf(u[i][2], gamma[i].z, beta[i].z));
-        dy[i][3] = through_activation<KIND>(dy[i][3], fmaf(u[i][3], gamma[i].w, beta[i].w));
+        through_activation<KIND>(pair(dy[i][0], dy[i][1]), fma(pair(u[i][0], u[i][1]), pair(gamma[i].x, gamma[i].y), pair(beta[i].x, beta[i].y))).get(dy[i][0], dy[i][1]);
+        through_activation<KIND>(pair(dy[i][2], dy[i][3]), fma(pair(u[i][2], u[i][3]), pair(gamma[i].z, gamma[i].w), pair(beta[i].z, beta[i].w))).get(dy[i][2], dy[i][3]);
     }
 }
 // Calls f with the epilogue as a constant: one branch for all that f does.
