@@ -20,11 +20,13 @@ template<int KIND, int Q>
 __device__ __forceinline__ void row_terms(float mean, float rstd, const float *gamma_at, int beta_at, const int (&at)[Q], float (&x)[Q][4], float (&dy)[Q][4],
                                           float (&dgamma)[Q][4], float (&dbeta)[Q][4], float (&sums)[2]) {
     float4 gamma[Q];
+    const pair minus_mean(-mean), scale(rstd);
+    pair sum_h(0.0f), sum_hu(0.0f);
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
         gamma[i] = *reinterpret_cast<const float4 *>(gamma_at + at[i]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[i][k] = (x[i][k] - mean) * rstd;
+        for (int k = 0; k < 4; k += 2) ((pair(x[i][k], x[i][k + 1]) + minus_mean) * scale).get(x[i][k], x[i][k + 1]);
     }
     if constexpr (KIND != CB200_EPILOGUE_NONE) {
         float4 beta[Q];
@@ -34,16 +36,19 @@ __device__ __forceinline__ void row_terms(float mean, float rstd, const float *g
     }
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-        const float g[4] = {gamma[i].x, gamma[i].y, gamma[i].z, gamma[i].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            dbeta[i][k] += dy[i][k];
-            dgamma[i][k] = fmaf(dy[i][k], x[i][k], dgamma[i][k]);
-            dy[i][k] *= g[k];
-            sums[0] += dy[i][k];
-            sums[1] = fmaf(dy[i][k], x[i][k], sums[1]);
+        for (int k = 0; k < 4; k += 2) {
+            const pair u(x[i][k], x[i][k + 1]), dz(dy[i][k], dy[i][k + 1]);
+            (pair(dbeta[i][k], dbeta[i][k + 1]) + dz).get(dbeta[i][k], dbeta[i][k + 1]);
+            fma(dz, u, pair(dgamma[i][k], dgamma[i][k + 1])).get(dgamma[i][k], dgamma[i][k + 1]);
+            const pair h = dz * (k == 0 ? pair(gamma[i].x, gamma[i].y) : pair(gamma[i].z, gamma[i].w));
+            sum_h = sum_h + h;
+            sum_hu = fma(h, u, sum_hu);
+            h.get(dy[i][k], dy[i][k + 1]);
         }
     }
+    sums[0] = sum_h.sum();
+    sums[1] = sum_hu.sum();
 }
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  Columns past the last hold
@@ -102,10 +107,12 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? 3 : 2) layer_norm
         sums[0] *= inverse;
         sums[1] *= inverse;
         if (!active || p.dx.base == nullptr) continue;
+        const pair scale(rstd), minus_h(-sums[0]), minus_hu(-sums[1]);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][k] = rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
+            for (int k = 0; k < 4; k += 2)
+                (scale * fma(pair(x[i][k], x[i][k + 1]), minus_hu, pair(dy[i][k], dy[i][k + 1]) + minus_h)).get(x[i][k], x[i][k + 1]);
         }
         store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, p.columns, p.per_access, p.dx.dtype, x);
     }
@@ -194,12 +201,12 @@ __global__ void __launch_bounds__(kBlockThreads) layer_norm_back_block_kernel(co
         sums[0] = lane < warps ? notes[set][0][lane] : 0.0f;
         sums[1] = lane < warps ? notes[set][1][lane] : 0.0f;
         warp_sums(sums);
-        sums[0] *= inverse;
-        sums[1] *= inverse;
+        const pair scale(rstd), minus_h(-sums[0] * inverse), minus_hu(-sums[1] * inverse);
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][k] = rstd * (dy[i][k] - sums[0] - x[i][k] * sums[1]);
+            for (int k = 0; k < 4; k += 2)
+                (scale * fma(pair(x[i][k], x[i][k + 1]), minus_hu, pair(dy[i][k], dy[i][k + 1]) + minus_h)).get(x[i][k], x[i][k + 1]);
         }
         store_quads<HALVES>(p.dx.base + row * p.dx.pitch, col, n, p.per_access, p.dx.dtype, x);
     }
