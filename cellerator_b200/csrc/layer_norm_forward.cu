@@ -39,39 +39,45 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm
     }
     __syncthreads();
     for (; row - group < p.rows; row += step) {
-        float v[ITEMS][4], sum[1] = {0.0f};
+        float v[ITEMS][4];
+        pair all(0.0f);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             raw[i].template widen<HALVES>(half, v[i]);
-            sum[0] += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+            all = all + (pair(v[i][0], v[i][1]) + pair(v[i][2], v[i][3]));
         }
+        float sum[1] = {all.sum()};
         if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
         lane_sums(sum, p.lanes);
         const float mean = sum[0] / count; // a division: exact for rows of one value
-        sum[0] = 0.0f;
+        const pair minus_mean(-mean);
+        all = pair(0.0f);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] -= mean;
+            for (int k = 0; k < 4; k += 2) (pair(v[i][k], v[i][k + 1]) + minus_mean).get(v[i][k], v[i][k + 1]);
             if (col[i] + 4 > p.columns) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (col[i] + k >= p.columns) v[i][k] = 0.0f;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[0] = fmaf(v[i][k], v[i][k], sum[0]);
+            for (int k = 0; k < 4; k += 2) {
+                const pair d(v[i][k], v[i][k + 1]);
+                all = fma(d, d, all);
+            }
         }
+        sum[0] = all.sum();
         lane_sums(sum, p.lanes);
         const float rstd = rsqrtf(fmaf(sum[0], inverse, p.epsilon));
         if (row >= p.rows) continue;
+        const pair scale(rstd);
         if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
             const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
-            v[i][0] = fmaf(v[i][0] * rstd, g.x, b.x);
-            v[i][1] = fmaf(v[i][1] * rstd, g.y, b.y);
-            v[i][2] = fmaf(v[i][2] * rstd, g.z, b.z);
-            v[i][3] = fmaf(v[i][3] * rstd, g.w, b.w);
+            fma(pair(v[i][0], v[i][1]) * scale, pair(g.x, g.y), pair(b.x, b.y)).get(v[i][0], v[i][1]);
+            fma(pair(v[i][2], v[i][3]) * scale, pair(g.z, g.w), pair(b.z, b.w)).get(v[i][2], v[i][3]);
         }
         activate(p.epilogue, v);
         drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
