@@ -151,7 +151,7 @@ def test_in_place(cuda_device, cols):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-@pytest.mark.parametrize("cols", [64, 5000])
+@pytest.mark.parametrize("cols", [64, 5000, 33_538, 40_000])
 def test_hard_rows(cuda_device, cols):
     """Rows of one value (with and without eps), far from zero, tiny and huge ones, and rows with an infinity or a NaN, whose
     neighbours are not touched.  A constant row whose mean is exact has u = 0 and the gradient of the formula."""
@@ -336,3 +336,40 @@ def test_more_than_2_to_the_32_bytes(cuda_device):
         assert_within(got[1], terms[0][1], terms[1][1], name="dgamma")
         assert_within(got[2], terms[0][2], terms[1][2], name="dbeta")
         del x, dy, got, stats
+
+
+@pytest.mark.parametrize("cols", [50, 1300, 9001, 40_001])
+def test_two_streams_at_once(cuda_device, cols):
+    """Calls that overlap on the device, each with memory of its own, give what they give one after the other."""
+    parameters_of = parameters(cols, cuda_device, 61)
+    inputs = [(matrix(700, cols, torch.float32, cuda_device, 62 + k), matrix(700, cols, torch.bfloat16, cuda_device, 64 + k)) for k in range(2)]
+    more = dict(epilogue="gelu_erf", dropout=0.25, seed=8)
+
+    def both(x, dy, sequence):
+        stats = torch.empty(700, 2, device=cuda_device)
+        y = ops.layer_norm(x, *parameters_of, stats=stats, sequence=sequence, **more)
+        return y, stats, *ops.layer_norm_backward(x, dy, stats, *parameters_of, sequence=sequence, **more)
+
+    want = [both(*inputs[k], k) for k in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k] = both(*inputs[k], k)
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want[k]))
+
+
+def test_gradients_of_parameters_that_were_not_given(cuda_device):
+    """dgamma and dbeta are sums over rows whether or not there is a gamma or a beta to move."""
+    for cols in (50, 1300, 5000):
+        x, dy = matrix(300, cols, torch.float32, cuda_device, 71), matrix(300, cols, torch.float32, cuda_device, 72)
+        stats = torch.empty(300, 2, device=cuda_device)
+        ops.layer_norm(x, stats=stats)
+        one, zero = torch.ones(cols, device=cuda_device), torch.zeros(cols, device=cuda_device)
+        want = ops.layer_norm_backward(x, dy, stats, one, zero)
+        got = ops.layer_norm_backward(x, dy, stats, dgamma=torch.full_like(one, 7.0), dbeta=torch.full_like(one, 7.0))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
