@@ -15,8 +15,8 @@ constexpr std::int64_t kNarrowColumns = 8 * 32 * 4;
 constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
-// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 71 us, 5.5 TB/s,
-// 84 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
+// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 70 us, 5.6 TB/s,
+// 86 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
 // once).  GELU and dropout are bound by instructions: 48 million values 90 us.
 template<int SIZE, bool HALVES, int ITEMS>
 __global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm_narrow_kernel(const layer_norm_params p) {

@@ -117,7 +117,8 @@ __device__ __forceinline__ void load4(const WT *p, float (&w)[4]) {
 // instructions (62 % of the slots, six for an entry in its share of a warp).  Before loads lost their branches 104 and 437.  Measured
 // against it: scales and zero-points in shared memory, with fewer blocks an SM, 112 and 430 us; a third stage of loads under way 84; rows
 // of A kept in L1 79 and 298; scales and zero-points side by side, laid so in a launch before, 77 and 305; parts of 256 entries 86 and
-// 369; four blocks an SM by launch bounds 93; every part's sum by a butterfly over all columns, and partial segments wholly in the
+// 369; four blocks an SM by launch bounds 93, and with four rows of A in flight instead of eight 85 and
+// 320; two blocks and sixteen rows 105 and 382; every part's sum by a butterfly over all columns, and partial segments wholly in the
 // branch that looks, 78 and 298.
 template<int BITS, typename WT, int V>
 __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
