@@ -161,14 +161,15 @@ constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
 constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
 
 // The quads of a thread lie a block's width apart; only the last of them can reach past the row's end.
-template<int SIZE, bool HALVES, int QT>
+// PLAIN: neither activation nor dropout (with the choices of them, which none of these rows needs, 6 % slower).
+template<int SIZE, bool HALVES, int QT, bool PLAIN>
 __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const layer_norm_params p, int beta_quads) {
     constexpr bool kAhead = QT * SIZE <= 16; // registers for two rows
     extern __shared__ __align__(16) float parameters[]; // gamma, then beta of each thread's first beta_quads quads
     __shared__ block_statistics statistics;
     const int n = p.columns, width = static_cast<int>(blockDim.x) * 4;
     const bool half = p.x.dtype == CB200_DTYPE_F16;
-    const std::uint64_t sequence = sequence_of(p.drop);
+    const std::uint64_t sequence = PLAIN ? 0u : sequence_of(p.drop);
     const int padded = (n + 3) & ~3;
     const float *beta_at = parameters + padded + 4; // behind each there is room for a quad past the row's end
     const bool beta_vectors = p.beta != nullptr && reinterpret_cast<std::uintptr_t>(p.beta) % 16u == 0u;
@@ -228,8 +229,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
                 v[j][2] = fmaf((v[j][2] - mean) * rstd, g.z, b[2]);
                 v[j][3] = fmaf((v[j][3] - mean) * rstd, g.w, b[3]);
             }
-            activate(p.epilogue, v);
-            drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), at, v);
+            if constexpr (!PLAIN) {
+                activate(p.epilogue, v);
+                drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), at, v);
+            }
             if (first + B < QT) store_quads<HALVES, B>(y, at, n, p.per_access, p.y.dtype, v);
             else store_quads<HALVES, B - 1>(y, at, n, p.per_access, p.y.dtype, v);
         }
@@ -242,9 +245,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
     }
 }
 
-template<int SIZE, bool HALVES, int QT>
+template<int SIZE, bool HALVES, int QT, bool PLAIN>
 cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t stream) {
-    constexpr auto kernel = layer_norm_row_kernel<SIZE, HALVES, QT>;
+    constexpr auto kernel = layer_norm_row_kernel<SIZE, HALVES, QT, PLAIN>;
     const int quads = (p.columns + 3) / 4, threads = ((quads + QT - 1) / QT + 31) / 32 * 32;
     const std::size_t gamma_bytes = static_cast<std::size_t>(quads + 1) * 16u, width = static_cast<std::size_t>(threads) * 16u;
     const std::size_t beta_quads = std::min<std::size_t>(QT, (kRowShared - gamma_bytes) / width), beta_bytes = beta_quads == QT ? gamma_bytes : beta_quads * width;
@@ -342,6 +345,11 @@ cb200_status launch_narrow(const layer_norm_params &p, cudaStream_t stream) {
     count_launch();
     CB200_CUDA_OK(cudaGetLastError());
     return CB200_STATUS_SUCCESS;
+}
+
+template<int SIZE, bool HALVES, int QT>
+cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t stream) {
+    return p.epilogue == CB200_EPILOGUE_NONE && !p.drop.on ? launch_rows<SIZE, HALVES, QT, true>(p, device, stream) : launch_rows<SIZE, HALVES, QT, false>(p, device, stream);
 }
 
 template<int SIZE, bool HALVES>

@@ -110,7 +110,8 @@ __device__ __forceinline__ void load4(const WT *p, float (&w)[4]) {
 // codes being on their way meanwhile; then `lanes` lanes serve an entry, V columns of A each, 8 rows of A in flight.  A part's sum is
 // that of 32 / lanes classes of its entries, a row's that of its parts in order, and the product with B follows from shared memory.
 // Lanes past a part's end read its last entry again, and genes outside the matrix row 0 of A: both are staged as gene -1, whose row
-// counts as zeros whatever it holds.  Segments without such entries, nearly all, take the branch that does not look.
+// counts as zeros whatever it holds.  Segments without such genes, up to the last whole piece of 8 entries a class, take the branch that
+// does not look.
 //
 // 4,099 x 33,538, 8 bits, rank 16 bf16: 75 us, bound by what the SMs get out of L2 in pieces of 32 bytes at random places (a row of A, a
 // scale and a zero-point for each entry).  50,000 x 4,000, 4 bits, rank 32: 292 us, bound by L1's wavefronts (72 %, two for an entry) and
