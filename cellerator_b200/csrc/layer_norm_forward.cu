@@ -151,17 +151,17 @@ __device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float cent
 
 // A block per row, the row in registers, its next row on the way where two fit and asked for in L2 where not; gamma and beta stay in
 // shared memory from row to row, as many columns of them as it holds (the rest of beta comes out of L2).
-// 4,099 x 33,538 bf16: 178 us, 47 % of a copy.  Half of the issue slots are taken (25 instructions a value; 41 with branches for each quad,
-// 277 us), and 30 warps, all at the same step of the same row, do not fill the others.  Measured against it: a cluster of eight blocks
+// 4,099 x 33,538 bf16: 158 us, 53 % of a copy.  Half of the issue slots are taken (some 20 instructions a value; 41 with branches for each
+// quad, 277 us), and 30 warps, all at the same step of the same row, do not fill the others.  Measured against it: a cluster of eight blocks
 // per row, whose threads kept gamma and beta of their columns, 373 us, waiting for its barriers; 512 threads with twice the quads 260;
-// the next row's quads loaded as soon as these are stored 180; one quad at a time, or two-wide products, 190 (spills); the
-// columns walked twice as below 212.
+// the next row's quads loaded as soon as these are stored 173; two-wide products 183 (registers); the choices of activation and
+// dropout in the loop 180; three quads at a time 169; the columns walked twice as below 212.
 constexpr int kRowThreads = 1024;
 constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
 constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
 
 // The quads of a thread lie a block's width apart; only the last of them can reach past the row's end.
-// PLAIN: neither activation nor dropout (with the choices of them, which none of these rows needs, 6 % slower).
+// PLAIN: neither activation nor dropout.
 template<int SIZE, bool HALVES, int QT, bool PLAIN>
 __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const layer_norm_params p, int beta_quads) {
     constexpr bool kAhead = QT * SIZE <= 16; // registers for two rows
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
         const float2 s = statistics.of_row(set, own_columns, own_inverse, centre, sums.moved.sum(), sums.spread.sum(), static_cast<float>(n), p.epsilon);
         const float mean = s.x, rstd = s.y;
         if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = s;
-        // a few quads at a time: what is computed takes twice the registers of what was loaded
-        constexpr int B = QT % 3 == 0 ? 3 : 2;
+        // a few quads at a time, so that one choice of activation serves them; more would not fit the registers
+        constexpr int B = PLAIN ? 1 : QT % 3 == 0 ? 3 : 2;
         unsigned char *y = p.y.base + row * p.y.pitch;
 #pragma unroll
         for (int first = 0; first < QT; first += B) {
