@@ -3,6 +3,7 @@
 // Mean and variance are sums in fp32 over values that stay in registers: the mean first, then the squares of what differs
 // from it, so that a row far from zero loses nothing.
 #include "layer_norm.cuh"
+#include "layer_norm_shapes.hh"
 
 #include <atomic>
 
@@ -10,7 +11,6 @@ namespace cb200 {
 namespace {
 
 constexpr int kNarrowItems[] = {4, 3, 2, 6, 8}; // quads of a row that a lane can hold, four by preference (32 columns: 65 us, eight 111)
-constexpr std::int64_t kNarrowColumns = 8 * 32 * 4;
 // Blocks that are resident on an SM.
 constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
@@ -156,11 +156,9 @@ __device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float cent
 // per row, whose threads kept gamma and beta of their columns, 373 us, waiting for its barriers; 512 threads with twice the quads 260;
 // the next row's quads loaded as soon as these are stored 173; two-wide products 183 (registers); the choices of activation and
 // dropout in the loop 180; three quads at a time 169; the columns walked twice as below 212.
-constexpr int kRowThreads = 1024;
-constexpr std::int64_t kRowColumns = 9 * 4 * kRowThreads; // 36,864
-constexpr std::size_t kRowShared = 220 * 1024;            // of parameters, at most
+constexpr std::size_t kRowShared = 220 * 1024; // of parameters, at most
 
-// The quads of a thread lie a block's width apart; only the last of them can reach past the row's end.
+// The quads of a thread lie a block's width apart; only the last of them can reach past the row's end (layer_norm_shapes.hh).
 // PLAIN: neither activation nor dropout.
 template<int SIZE, bool HALVES, int QT, bool PLAIN>
 __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const layer_norm_params p, int beta_quads) {
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
 template<int SIZE, bool HALVES, int QT, bool PLAIN>
 cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t stream) {
     constexpr auto kernel = layer_norm_row_kernel<SIZE, HALVES, QT, PLAIN>;
-    const int quads = (p.columns + 3) / 4, threads = ((quads + QT - 1) / QT + 31) / 32 * 32;
+    const int quads = (p.columns + 3) / 4, threads = row_threads_of(p.columns);
     const std::size_t gamma_bytes = static_cast<std::size_t>(quads + 1) * 16u, width = static_cast<std::size_t>(threads) * 16u;
     const std::size_t beta_quads = std::min<std::size_t>(QT, (kRowShared - gamma_bytes) / width), beta_bytes = beta_quads == QT ? gamma_bytes : beta_quads * width;
     // more than the default 48 KB is asked for once per kernel and device
@@ -355,7 +353,7 @@ cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t st
 
 template<int SIZE, bool HALVES>
 cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream) {
-    if (p.columns <= kNarrowColumns) {
+    if (p.columns <= kWarpColumns) {
         const narrow_shape narrow = narrow_shape_of(p.columns, kNarrowItems, 5);
         p.lanes = narrow.lanes;
         switch (narrow.items) {
@@ -366,12 +364,14 @@ cb200_status launch_forward(layer_norm_params p, int device, cudaStream_t stream
         default: return launch_narrow<SIZE, HALVES, 8>(p, stream);
         }
     }
-    // quads of a thread: all but its last lie in the row, with blocks that are a multiple of 32 threads, from 64 quads on with two,
-    // 376 with four, 937 with six and 2,520 with nine
-    if (p.columns <= 2048) return launch_rows<SIZE, HALVES, 2>(p, device, stream);
-    if (p.columns <= 4 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 4>(p, device, stream);
-    if (p.columns <= 6 * 4 * kRowThreads) return launch_rows<SIZE, HALVES, 6>(p, device, stream);
-    if (p.columns <= kRowColumns) return launch_rows<SIZE, HALVES, 9>(p, device, stream);
+    if (p.columns <= kRowColumns) {
+        switch (row_quads_of(p.columns)) {
+        case 2: return launch_rows<SIZE, HALVES, 2>(p, device, stream);
+        case 4: return launch_rows<SIZE, HALVES, 4>(p, device, stream);
+        case 6: return launch_rows<SIZE, HALVES, 6>(p, device, stream);
+        default: return launch_rows<SIZE, HALVES, 9>(p, device, stream);
+        }
+    }
     layer_norm_long_kernel<SIZE, HALVES><<<static_cast<unsigned>(std::min<std::int64_t>(p.rows, 148 * 2)), kLongThreads, 0, stream>>>(p);
     count_launch();
     CB200_CUDA_OK(cudaGetLastError());
