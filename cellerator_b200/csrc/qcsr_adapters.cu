@@ -2,6 +2,7 @@
 //     out[r] = act(alpha s_a (deq(X)[r] A_a) B_a + beta out[r] + bias),  a = adapter[r].
 // The same walk over the row's entries as the projection, with a narrow operand that changes from row to row, and the second
 // product while the first is still in shared memory.
+#include "adapter_parts.hh"
 #include "kernels.cuh"
 
 #include <algorithm>
@@ -11,9 +12,6 @@
 namespace cb200 {
 namespace {
 
-constexpr int kRuns = 4;                // runs of 32 entries that a warp decodes at a time
-constexpr int kSegment = 32 * kRuns;
-constexpr int kMostParts = 32;          // of a row
 constexpr int kWarps = 8;
 constexpr int kMostRows = 8;            // of a block
 constexpr int kMostRank = 256;
@@ -37,12 +35,6 @@ struct adapter_params {
     int up_quads;   // B in columns of four
     int block_rows; // rows of a block
 };
-
-// Entries of a part of a row of `len` entries, a multiple of a warp's segment: by the length alone.
-__device__ __forceinline__ int part_entries(int len) {
-    const int even = (len + kMostParts - 1) / kMostParts;
-    return max(kSegment, (even + kSegment - 1) / kSegment * kSegment);
-}
 
 // V neighbouring elements of a row of A.
 template<typename WT, int V>
@@ -125,7 +117,8 @@ template<int BITS, typename WT, int V>
 __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter_params p) {
     __shared__ __align__(16) int2 staged[kWarps][kSegment];
     __shared__ std::int64_t row_start[kMostRows], code_start[kMostRows];
-    __shared__ int row_len[kMostRows], row_share[kMostRows], row_adapter[kMostRows], first_part[kMostRows + 1];
+    __shared__ unsigned row_len[kMostRows], row_share[kMostRows];
+    __shared__ int row_adapter[kMostRows], first_part[kMostRows + 1];
     extern __shared__ float sums[]; // [parts][rank]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const std::int64_t row0 = p.row_begin + static_cast<std::int64_t>(blockIdx.x) * p.block_rows;
@@ -136,13 +129,13 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
             const int a = __ldg(p.adapter + row0 + lane);
             const bool has = a >= 0 && a < p.adapters && p.cols > 0;
             const std::int64_t start = __ldg(p.row_ptr + row0 + lane);
-            const int len = has ? static_cast<int>(__ldg(p.row_ptr + row0 + lane + 1) - start) : 0, share = part_entries(len);
+            const unsigned len = has ? static_cast<unsigned>(__ldg(p.row_ptr + row0 + lane + 1) - start) : 0u, share = part_entries(len);
             row_adapter[lane] = has ? a : -1;
             row_start[lane] = start;
             row_len[lane] = len;
             row_share[lane] = share;
             code_start[lane] = p.packed_row_ptr != nullptr ? __ldg(p.packed_row_ptr + row0 + lane) : start;
-            upto = (len + share - 1) / share;
+            upto = static_cast<int>(parts_of(len, share));
         }
 #pragma unroll
         for (int off = 1; off < kMostRows; off <<= 1) {
@@ -162,13 +155,14 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
     for (int column0 = 0; column0 < p.rank; column0 += lanes * V) { // of A; one turn but for wide ranks of narrow slices
         const int col = column0 + in_row * V;
         const bool holds = col < p.rank;
-        int part = warp, r = 0, at = 0, to = 0; // entries of row r: those of the segment start at `at`
+        int part = warp, r = 0;
+        unsigned at = 0, to = 0; // entries of row r: those of the segment start at `at`
         int gene[kRuns];
         unsigned code[kRuns];
         const auto fetch = [&]() {
             const std::int32_t *cols = p.col_idx + row_start[r] + at;
             const std::uint8_t *codes = p.packed + code_start[r] + (BITS == 8 ? at : at >> 1); // `at` is even
-            const int last = to - at - 1;
+            const int last = static_cast<int>(to - at) - 1;
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) {
                 const int e = min(i * 32 + lane, last);
@@ -180,8 +174,8 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
         const auto open = [&]() {
             if (part >= parts) return;
             r = __popc(__ballot_sync(0xffffffffu, lane < rows && first_part[min(lane, kMostRows)] <= part)) - 1;
-            at = (part - first_part[r]) * row_share[r];
-            to = min(row_len[r], at + row_share[r]);
+            at = static_cast<unsigned>(part - first_part[r]) * row_share[r];
+            to = part_end(at, row_len[r], row_share[r]);
             fetch();
         };
         open();
@@ -189,7 +183,7 @@ __global__ void __launch_bounds__(kWarps * 32) qcsr_adapter_kernel(const adapter
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
         while (part < parts) {
-            const int count = min(kSegment, to - at), part_now = part;
+            const int count = static_cast<int>(min(static_cast<unsigned>(kSegment), to - at)), part_now = part;
             const unsigned char *down = p.down + static_cast<std::int64_t>(row_adapter[r]) * p.cols * row_bytes + (holds ? col : 0) * sizeof(WT);
             float scale[kRuns], offset[kRuns];
             bool fine = holds;
