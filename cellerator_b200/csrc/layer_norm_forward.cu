@@ -1,7 +1,7 @@
 // Layer norm over the rows of a dense matrix, with the activation and the dropout that follow it in the same pass:
 //     u = (x - mean) / sqrt(var + eps),  y = drop(act(gamma u + beta)).
-// Mean and variance are sums in fp32 over values that stay in registers: the mean first, then the squares of what differs
-// from it, so that a row far from zero loses nothing.
+// Mean and variance are sums in fp32 over values that stay in registers, of what the values differ from a number next to their mean, so
+// that a row far from zero loses what its mean's own rounding takes, and a row of one value is beta.
 #include "layer_norm.cuh"
 #include "layer_norm_shapes.hh"
 
@@ -14,122 +14,7 @@ constexpr int kNarrowItems[] = {4, 3, 2, 6, 8}; // quads of a row that a lane ca
 // Blocks that are resident on an SM.
 constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
-// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
-// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 70 us, 5.6 TB/s,
-// 86 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
-// once).  GELU and dropout are bound by instructions: 48 million values 90 us.
-template<int SIZE, bool HALVES, int ITEMS>
-__global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm_narrow_kernel(const layer_norm_params p) {
-    constexpr int kColumns = ITEMS * 32 * 4 + 4;
-    __shared__ __align__(16) float parameters[2][kColumns];
-    const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
-    const bool half = p.x.dtype == CB200_DTYPE_F16;
-    const std::uint64_t sequence = sequence_of(p.drop);
-    int col[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
-    const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
-    const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
-    std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
-    raw_quad<SIZE> raw[ITEMS];
-    if (row < p.rows) load_quads(p.x.base + row * p.x.pitch, col, p.columns, p.per_access, raw);
-    for (int c = threadIdx.x; c < kColumns; c += kNarrowThreads) {
-        parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
-        parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
-    }
-    __syncthreads();
-    for (; row - group < p.rows; row += step) {
-        float v[ITEMS][4];
-        pair all(0.0f);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            raw[i].template widen<HALVES>(half, v[i]);
-            all = all + (pair(v[i][0], v[i][1]) + pair(v[i][2], v[i][3]));
-        }
-        float sum[1] = {all.sum()};
-        if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
-        lane_sums(sum, p.lanes);
-        const float mean = sum[0] / count; // a division: exact for rows of one value
-        const pair minus_mean(-mean);
-        all = pair(0.0f);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) (pair(v[i][k], v[i][k + 1]) + minus_mean).get(v[i][k], v[i][k + 1]);
-            if (col[i] + 4 > p.columns) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (col[i] + k >= p.columns) v[i][k] = 0.0f;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-                const pair d(v[i][k], v[i][k + 1]);
-                all = fma(d, d, all);
-            }
-        }
-        sum[0] = all.sum();
-        lane_sums(sum, p.lanes);
-        const float rstd = rsqrtf(fmaf(sum[0], inverse, p.epsilon));
-        if (row >= p.rows) continue;
-        const pair scale(rstd);
-        if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
-            const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
-            fma(pair(v[i][0], v[i][1]) * scale, pair(g.x, g.y), pair(b.x, b.y)).get(v[i][0], v[i][1]);
-            fma(pair(v[i][2], v[i][3]) * scale, pair(g.z, g.w), pair(b.z, b.w)).get(v[i][2], v[i][3]);
-        }
-        activate(p.epilogue, v);
-        drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
-        store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
-    }
-}
-
-// Mean and variance of a row that a block's threads hold, in one walk over the values and with one barrier.  Each thread sums up
-// its columns' distances from a centre of its own, the mean of its first quad, and their squares: the square of how far that is
-// from the mean of all its columns is at most the number of its quads times their variance, so no digits are lost to the difference
-// in the end.  From {sum, squares about its mean} of each thread come those of the warps, and from these
-//     mean = sum of sums / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2).
-struct block_statistics {
-    float notes[2][2][32], sizes[32], inverses[32]; // of the warps: of two rows in turn; columns
-
-    // before the first row; own: columns of the thread
-    __device__ __forceinline__ void begin(float own) {
-        float size[1] = {own};
-        warp_sums(size);
-        if ((threadIdx.x & 31) == 0) {
-            sizes[threadIdx.x >> 5] = size[0];
-            inverses[threadIdx.x >> 5] = size[0] > 0.0f ? 1.0f / size[0] : 0.0f;
-        }
-        __syncwarp();
-    }
-    // {mean, 1 / sqrt(var + epsilon)}.  moved, spread: sums of the thread's distances from `centre` and of their squares.
-    __device__ __forceinline__ float2 of_row(int set, float own, float own_inverse, float centre, float moved, float spread, float count, float epsilon) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        float t[1] = {fmaf(own, centre, moved)};
-        const float off = moved * own_inverse; // of the thread's mean from its centre
-        warp_sums(t);
-        if (lane == 0) notes[set][0][warp] = t[0];
-        const float differs = (centre - t[0] * inverses[warp]) + off;
-        t[0] = fmaf(own * differs, differs, fmaf(-moved, off, spread));
-        warp_sums(t);
-        if (lane == 0) notes[set][1][warp] = t[0];
-        __syncthreads();
-        const float of_warp = lane < warps ? notes[set][0][lane] : 0.0f;
-        t[0] = of_warp;
-        warp_sums(t);
-        const float mean = t[0] / count; // a division: exact for rows of one value
-        t[0] = 0.0f;
-        if (lane < warps) {
-            const float from = fmaf(of_warp, inverses[lane], -mean);
-            t[0] = fmaf(sizes[lane] * from, from, notes[set][1][lane]);
-        }
-        warp_sums(t);
-        return make_float2(mean, rsqrtf(fmaf(t[0], 1.0f / count, epsilon)));
-    }
-};
-
-// The sums of a thread's distances from its centre, a quad at a time.
+// The sums of a thread's distances from its centre and of their squares, a quad at a time.
 struct thread_statistics {
     pair minus, moved, spread;
     __device__ __forceinline__ explicit thread_statistics(float centre) : minus(-centre), moved(0.0f), spread(0.0f) {}
@@ -148,6 +33,151 @@ __device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float cent
     for (int k = 0; k < 4; ++k)
         if (at + k >= n) v[k] = centre;
 }
+
+// A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
+// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 70 us, 5.6 TB/s,
+// 86 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
+// once).  GELU and dropout are bound by instructions: 48 million values 90 us.
+// Of fp32 rows a lane sums up distances from its first value, and the lanes' sums meet as distances from the first lane's: all of them zero in
+// a row of one value.  The sum of the values themselves is rounded, which such a row, if its value is large, shows as that rounding over
+// sqrt(epsilon).  Rows of 16-bit values need it not: the sum of 1,024 equal ones is a number of fp32.
+template<int SIZE, bool HALVES, int ITEMS>
+__global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm_narrow_kernel(const layer_norm_params p) {
+    constexpr int kColumns = ITEMS * 32 * 4 + 4;
+    constexpr bool kCentred = SIZE == 4;
+    __shared__ __align__(16) float parameters[2][kColumns];
+    const int lane = threadIdx.x & 31, in_row = lane & (p.lanes - 1), group = lane / p.lanes, rows_per_warp = 32 / p.lanes;
+    const bool half = p.x.dtype == CB200_DTYPE_F16;
+    const std::uint64_t sequence = sequence_of(p.drop);
+    int col[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) col[i] = min((i * p.lanes + in_row) * 4, (p.columns + 3) & ~3);
+    const float count = static_cast<float>(p.columns), inverse = 1.0f / count;
+    const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * (kNarrowThreads / 32) * rows_per_warp;
+    std::int64_t row = (static_cast<std::int64_t>(blockIdx.x) * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * rows_per_warp + group;
+    raw_quad<SIZE> raw[ITEMS];
+    if (row < p.rows) load_quads(p.x.base + row * p.x.pitch, col, p.columns, p.per_access, raw);
+    for (int c = threadIdx.x; c < kColumns; c += kNarrowThreads) {
+        parameters[0][c] = p.gamma != nullptr && c < p.columns ? __ldg(p.gamma + c) : 1.0f;
+        parameters[1][c] = p.beta != nullptr && c < p.columns ? __ldg(p.beta + c) : 0.0f;
+    }
+    __syncthreads();
+    float own = 0.0f; // columns of the lane
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) own += static_cast<float>(min(max(p.columns - col[i], 0), 4));
+    const float own_inverse = own > 0.0f ? 1.0f / own : 0.0f;
+    for (; row - group < p.rows; row += step) {
+        float v[ITEMS][4], mean, rstd;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) raw[i].template widen<HALVES>(half, v[i]);
+        if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
+        if constexpr (kCentred) {
+            const float centre = v[0][0];
+            thread_statistics sums(centre);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                cut_off(v[i], col[i], p.columns, centre);
+                sums.add(v[i]);
+            }
+            const float first = __shfl_sync(0xffffffffu, centre, lane - in_row), moved = sums.moved.sum(), off = moved * own_inverse;
+            float t[1] = {fmaf(own, centre - first, moved)};
+            lane_sums(t, p.lanes);
+            mean = fmaf(t[0], inverse, first);
+            const float differs = (centre - mean) + off;
+            t[0] = fmaf(own * differs, differs, fmaf(-moved, off, sums.spread.sum()));
+            lane_sums(t, p.lanes);
+            rstd = rsqrtf(fmaf(t[0], inverse, p.epsilon));
+            const pair minus_mean(-mean);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) (pair(v[i][k], v[i][k + 1]) + minus_mean).get(v[i][k], v[i][k + 1]);
+            }
+        } else {
+            pair all(0.0f);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) all = all + (pair(v[i][0], v[i][1]) + pair(v[i][2], v[i][3]));
+            float sum[1] = {all.sum()};
+            lane_sums(sum, p.lanes);
+            mean = sum[0] / count; // a division: exact for rows of one value
+            const pair minus_mean(-mean);
+            all = pair(0.0f);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) (pair(v[i][k], v[i][k + 1]) + minus_mean).get(v[i][k], v[i][k + 1]);
+                cut_off(v[i], col[i], p.columns, 0.0f);
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                    const pair d(v[i][k], v[i][k + 1]);
+                    all = fma(d, d, all);
+                }
+            }
+            sum[0] = all.sum();
+            lane_sums(sum, p.lanes);
+            rstd = rsqrtf(fmaf(sum[0], inverse, p.epsilon));
+        }
+        if (row >= p.rows) continue;
+        const pair scale(rstd);
+        if (p.stats != nullptr && in_row == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) { // past the row's end there is room in the shared memory, and nothing is stored
+            const float4 g = *reinterpret_cast<const float4 *>(parameters[0] + col[i]), b = *reinterpret_cast<const float4 *>(parameters[1] + col[i]);
+            fma(pair(v[i][0], v[i][1]) * scale, pair(g.x, g.y), pair(b.x, b.y)).get(v[i][0], v[i][1]);
+            fma(pair(v[i][2], v[i][3]) * scale, pair(g.z, g.w), pair(b.z, b.w)).get(v[i][2], v[i][3]);
+        }
+        activate(p.epilogue, v);
+        drop_quads(p.drop, sequence, static_cast<std::uint32_t>(row), col, v);
+        store_quads<HALVES>(p.y.base + row * p.y.pitch, col, p.columns, p.per_access, p.y.dtype, v);
+    }
+}
+
+// Mean and variance of a row that a block's threads hold, in one walk over the values and with one barrier.  Each thread sums up
+// its columns' distances from a centre of its own, the mean of its first quad, and their squares: the square of how far that is
+// from the mean of all its columns is at most the number of its quads times their variance, so no digits are lost to the difference
+// in the end.  From the sum of each thread's distances and their squares about its mean come those of the warps, and from these
+//     mean = m0 + sum over warps of n (warp's mean - m0) / N,  N var = sum over warps of (squares + n (warp's mean - mean)^2),
+// m0 the first warp's mean; a warp's mean comes from its threads in the same way, from its first thread's centre on.  So what is summed up
+// are differences, all of them zero in a row of one value, and the mean of a row far from zero is off by roundings of itself alone.
+struct block_statistics {
+    float notes[2][2][32], sizes[32], inverses[32]; // of the warps: of two rows in turn, {mean, squares about it}; columns
+
+    // before the first row; own: columns of the thread
+    __device__ __forceinline__ void begin(float own) {
+        float size[1] = {own};
+        warp_sums(size);
+        if ((threadIdx.x & 31) == 0) {
+            sizes[threadIdx.x >> 5] = size[0];
+            inverses[threadIdx.x >> 5] = size[0] > 0.0f ? 1.0f / size[0] : 0.0f;
+        }
+        __syncwarp();
+    }
+    // {mean, 1 / sqrt(var + epsilon)}.  moved, spread: sums of the thread's distances from `centre` and of their squares.
+    __device__ __forceinline__ float2 of_row(int set, float own, float own_inverse, float centre, float moved, float spread, float count, float epsilon) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        const float first = __shfl_sync(0xffffffffu, centre, 0);
+        float t[1] = {fmaf(own, centre - first, moved)};
+        const float off = moved * own_inverse; // of the thread's mean from its centre
+        warp_sums(t);
+        const float of_mine = fmaf(t[0], inverses[warp], first);
+        if (lane == 0) notes[set][0][warp] = of_mine;
+        const float differs = (centre - of_mine) + off;
+        t[0] = fmaf(own * differs, differs, fmaf(-moved, off, spread));
+        warp_sums(t);
+        if (lane == 0) notes[set][1][warp] = t[0];
+        __syncthreads();
+        const float m0 = notes[set][0][0];
+        float from = lane < warps ? notes[set][0][lane] - m0 : 0.0f;
+        t[0] = lane < warps ? sizes[lane] * from : 0.0f;
+        warp_sums(t);
+        const float shift = t[0] / count;
+        from -= shift;
+        t[0] = lane < warps ? fmaf(sizes[lane] * from, from, notes[set][1][lane]) : 0.0f;
+        warp_sums(t);
+        const float mean = m0 + shift, inverse = 1.0f / count;
+        return make_float2(mean, rsqrtf(fmaf(t[0], inverse, epsilon)));
+    }
+};
 
 // A block per row, the row in registers, its next row on the way where two fit and asked for in L2 where not; gamma and beta stay in
 // shared memory from row to row, as many columns of them as it holds (the rest of beta comes out of L2).
