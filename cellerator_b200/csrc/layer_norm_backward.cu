@@ -325,7 +325,10 @@ extern "C" cb200_status cb200_layer_norm_backward(const cb200_layer_norm *d, voi
     if (d->stats == nullptr && p.rows > 0) return fail(CB200_STATUS_INVALID_ARGUMENT, "the backward pass needs the statistics of the forward pass");
     if (!rows_compatible(p.dx, p.x, p.rows, p.columns) || !rows_compatible(p.dx, p.dy, p.rows, p.columns))
         return fail(CB200_STATUS_INVALID_ARGUMENT, "dx overlaps x or dy without being it");
-    if (d->dgamma != nullptr && d->dgamma == d->dbeta) return fail(CB200_STATUS_INVALID_ARGUMENT, "dgamma and dbeta are the same vector");
+    if (d->dgamma != nullptr && d->dbeta != nullptr) {
+        const auto g = reinterpret_cast<std::uintptr_t>(d->dgamma), b = reinterpret_cast<std::uintptr_t>(d->dbeta);
+        if ((g > b ? g - b : b - g) < static_cast<std::uintptr_t>(d->columns) * sizeof(float)) return fail(CB200_STATUS_INVALID_ARGUMENT, "dgamma and dbeta overlap");
+    }
     const bool sums = d->dgamma != nullptr || d->dbeta != nullptr;
     const bool two_passes = p.columns > kBlockColumns && p.dx.base != nullptr;
     float *row_sums = nullptr;

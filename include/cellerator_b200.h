@@ -720,7 +720,7 @@ cb200_status cb200_dropout_rows(const cb200_dropout_matrix *matrix, void *stream
  * bias).  1 to 65,536 columns, fewer than 2^32 rows; more are refused.
  * Forward writes y (which may be x, as for dropout) and, when asked, stats.
  * Backward reads x, dy and the stats of the forward call with the same parameters, epilogue and dropout, and writes
- * those of dx (which may be x or dy), dgamma and dbeta that are not NULL; relu's slope is 0 at 0.  It needs
+ * those of dx (which may be x or dy), dgamma and dbeta (which share no byte) that are not NULL; relu's slope is 0 at 0.  It needs
  * cb200_layer_norm_backward_workspace bytes (4-byte aligned): two sums per column of every part that the rows are cut
  * into, which a last launch adds up in a fixed order, and above 4,608 columns two sums per row and 4,096 of its
  * columns.  Up to there dx alone needs none. */
