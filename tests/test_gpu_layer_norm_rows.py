@@ -95,3 +95,67 @@ def test_rows_far_from_zero(cuda_device, cols, far):
     x = matrix(90, cols, torch.float32, cuda_device, 7, 1.0, far)
     gamma, beta = parameters(cols, cuda_device, 8)
     check(x, gamma, beta)
+
+
+@pytest.mark.parametrize("kind,p", [("none", 0.0), ("relu", 0.0), ("gelu_erf", 0.2), ("gelu_tanh", 0.0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols,rows", [(1025, 2600), (2048, 1300), (2049, 1300), (4001, 700), (9000, 500), (16_384, 470), (16_386, 460), (24_576, 450), (24_577, 460), (33_538, 600),
+                                       (36_864, 450), (36_865, 620), (40_002, 620), (65_535, 600)])
+def test_blocks_that_take_several_rows(cuda_device, cols, rows, dtype, kind, p):
+    """At least three rows for a block, whose next one is loaded, or asked for, while one is worked on: each of them against the
+    definition, and with the bits that it has in shards of fewer rows than there are blocks."""
+    x = matrix(rows, cols, dtype, cuda_device, cols, 1.5, 0.25)
+    x[rows // 2:] -= 3.0                                            # the rows of a block are not alike
+    gamma, beta = parameters(cols, cuda_device, cols + 1)
+    y, stats = check(x, gamma, beta, kind, p, out_dtype=torch.float32)
+    for lo in range(0, rows, 140):
+        hi = min(rows, lo + 140)
+        some = torch.empty(hi - lo, 2, device=cuda_device)
+        assert torch.equal(ops.layer_norm(x[lo:hi], gamma, beta, epilogue=kind, dropout=p, seed=5, sequence=9, first_row=lo, out_dtype=torch.float32, stats=some), y[lo:hi])
+        assert torch.equal(some, stats[lo:hi])
+
+
+@pytest.mark.parametrize("kind", ["none", "relu", "gelu_erf", "gelu_tanh"])
+@pytest.mark.parametrize("cols,pitch,shift", [(1237, 1240, 1), (9001, 9001, 0), (33_538, 33_539, 1), (36_601, 36_601, 0), (36_867, 36_867, 3), (36_870, 36_872, 2), (40_001, 40_004, 0),
+                                              (65_533, 65_536, 4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_odd_places_of_wide_rows(cuda_device, cols, pitch, shift, dtype, kind):
+    """Rows of any width that start anywhere, parameters that start on no 16-byte boundary, one of them or none; what lies between the rows
+    stays as it was."""
+    x = matrix(9, cols, dtype, cuda_device, 11, 2.0, 0.5, pitch, shift)
+    buffer = matrix(1, 2 * cols + 3, torch.float32, cuda_device, 12, 0.3, 0.5)[0]
+    out = matrix(9, cols, dtype, cuda_device, 13, pitch=pitch, shift=shift)
+    one, zero = torch.ones(cols, device=cuda_device), torch.zeros(cols, device=cuda_device)
+    around = out._base.clone()
+    for gamma, beta in ((buffer[1:cols + 1], buffer[cols + 2:2 * cols + 2]), (buffer[:cols], None), (None, buffer[3:cols + 3]), (None, None)):
+        stats = torch.full((9, 2), float("nan"), device=cuda_device)
+        ops.layer_norm(x, gamma, beta, epilogue=kind, dropout=0.1, seed=5, sequence=9, out=out, stats=stats)
+        factor = keep(9, cols, 0.1, 5, 9, device=cuda_device).double() / 0.9
+        want, want_stats, bound, stats_bound = expected(x.double(), (one if gamma is None else gamma).double(), (zero if beta is None else beta).double(), 1e-5, kind, factor)
+        assert_within(out, want, bound, dtype, "y")
+        assert_within(stats, want_stats, stats_bound, name="stats")
+    out.copy_(around[shift:shift + 9 * pitch].view(9, pitch)[:, :cols])
+    assert torch.equal(out._base.view(torch.uint8), around.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [(3_000_000, 50, torch.float32), (400_000, 512, torch.bfloat16), (120_000, 2000, torch.bfloat16), (40_000, 4608, torch.float16)])
+def test_gradients_of_parameters_over_many_rows(cuda_device, rows, cols, dtype):
+    """Threads that add up the terms of hundreds of rows.  There are at least 148 blocks, so that no chain is longer than a 148th of the rows,
+    and 64 steps more join them; terms themselves are off as in norm_backward (row_operators.py): u by 2 U |u|, a product by U.  dy and the
+    terms of dgamma are not centred, so that the sums are of the size of their terms' sum."""
+    x = torch.randn(rows, cols, generator=torch.Generator(device=cuda_device).manual_seed(1), device=cuda_device).to(dtype)
+    dy = x.abs() + 0.25 * x                                         # dz u = |x| u + x u / 4
+    gamma, beta = parameters(cols, cuda_device, 15)
+    stats = torch.empty(rows, 2, device=cuda_device)
+    ops.layer_norm(x, gamma, beta, stats=stats)
+    _, dgamma, dbeta = ops.layer_norm_backward(x, dy, stats, gamma, beta, dx=dy.clone())
+    sums = [torch.zeros(cols, dtype=torch.float64, device=cuda_device) for _ in range(4)]
+    step = 32_000_000 // cols
+    for lo in range(0, rows, step):
+        s, d = stats[lo:lo + step].double(), dy[lo:lo + step].double()
+        terms = d * ((x[lo:lo + step].double() - s[:, :1]) * s[:, 1:])
+        for total, t in zip(sums, (terms, terms.abs(), d, d.abs())):
+            total += t.sum(0)
+    chain = rows / 148 + 64
+    assert_within(dgamma, sums[0], (chain + 4) * U * sums[1], name="dgamma")
+    assert_within(dbeta, sums[2], (chain + 1) * U * sums[3], name="dbeta")
