@@ -14,6 +14,9 @@ constexpr int kNarrowItems[] = {4, 3, 2, 6, 8}; // quads of a row that a lane ca
 // Blocks that are resident on an SM.
 constexpr int narrow_blocks(int items) { return items <= 4 ? 3 : 2; }
 
+// What a thread's distances are taken from, next to the value given.  Values too large for that (an infinity among them) keep their distance
+// from zero: 65,536 distances from 10^33 add up to a number of fp32 where the values do.
+__device__ __forceinline__ float centre_at(float v) { return fabsf(v) < 1e33f ? v : 0.0f; }
 // The sums of a thread's distances from its centre and of their squares, a quad at a time.
 struct thread_statistics {
     pair minus, moved, spread;
@@ -72,7 +75,7 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS <= 4 ? 3 : 2) layer_norm
         for (int i = 0; i < ITEMS; ++i) raw[i].template widen<HALVES>(half, v[i]);
         if (row + step < p.rows) load_quads(p.x.base + (row + step) * p.x.pitch, col, p.columns, p.per_access, raw);
         if constexpr (kCentred) {
-            const float centre = v[0][0];
+            const float centre = centre_at(v[0][0]);
             thread_statistics sums(centre);
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
@@ -168,14 +171,13 @@ struct block_statistics {
         __syncthreads();
         const float m0 = notes[set][0][0];
         float from = lane < warps ? notes[set][0][lane] - m0 : 0.0f;
-        t[0] = lane < warps ? sizes[lane] * from : 0.0f;
+        t[0] = lane < warps ? sizes[lane] / count * from : 0.0f; // shares, whose sum is a number of fp32 where the means are
         warp_sums(t);
-        const float shift = t[0] / count;
-        from -= shift;
+        const float mean = m0 + t[0];
+        from -= t[0];
         t[0] = lane < warps ? fmaf(sizes[lane] * from, from, notes[set][1][lane]) : 0.0f;
         warp_sums(t);
-        const float mean = m0 + shift, inverse = 1.0f / count;
-        return make_float2(mean, rsqrtf(fmaf(t[0], inverse, epsilon)));
+        return make_float2(mean, rsqrtf(fmaf(t[0], 1.0f / count, epsilon)));
     }
 };
 
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) layer_norm_row_kernel(const la
         }
         float v[4];
         now[0].template widen<HALVES>(half, v);
-        const float centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
+        const float centre = centre_at(0.25f * ((v[0] + v[1]) + (v[2] + v[3])));
         thread_statistics sums(centre);
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) layer_norm_long_kernel(const 
                 float v[4];
                 raw[i].template widen<HALVES>(half, v);
                 if (i == 0 && at == first) {
-                    centre = 0.25f * ((v[0] + v[1]) + (v[2] + v[3]));
+                    centre = centre_at(0.25f * ((v[0] + v[1]) + (v[2] + v[3])));
                     sums.minus = pair(-centre);
                 }
                 cut_off(v, col[i], n, centre);

@@ -719,6 +719,8 @@ cb200_status cb200_dropout_rows(const cb200_dropout_matrix *matrix, void *stream
  * var the mean of the squared differences.  epilogue: CB200_EPILOGUE_NONE, _RELU, _GELU_ERF or _GELU_TANH (beta is the
  * bias).  1 to 65,536 columns, fewer than 2^32 rows; more are refused.
  * Forward writes y (which may be x, as for dropout) and, when asked, stats.
+ * A row of one value has u = 0.  Squares and sums are fp32: a row whose variance passes its range (values that differ by 10^19)
+ * has 1 / sigma = 0, which makes u 0 as well, and one whose sum does is NaN.
  * Backward reads x, dy and the stats of the forward call with the same parameters, epilogue and dropout, and writes
  * those of dx (which may be x or dy), dgamma and dbeta (which share no byte) that are not NULL; relu's slope is 0 at 0.  It needs
  * cb200_layer_norm_backward_workspace bytes (4-byte aligned): two sums per column of every part that the rows are cut

@@ -97,6 +97,29 @@ def test_rows_far_from_zero(cuda_device, cols, far):
     check(x, gamma, beta)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [3, 50, 64, 512, 1000, 1025, 2049, 5000, 16_386, 33_538, 36_868, 40_001])
+def test_rows_with_a_huge_value(cuda_device, cols, dtype):
+    """One value whose square is no number of fp32, first, in the middle, in a thread's first four or last: the variance is infinite, 1 / sigma
+    zero, the row beta, and the mean the value's share.  Two of 3e38 have an infinite sum: their row is NaN, its neighbours are not."""
+    values = [1e20, -1e30, 2e33, 1e34, -3e36, 3.3e38, float(torch.finfo(dtype).min)]
+    places = sorted({0, 1 % cols, 2, cols // 2, cols - 1})
+    x = matrix(len(values) * len(places) + 3, cols, dtype, cuda_device, 21)
+    x[-2, :2] = 3e38
+    for i, value in enumerate(values):
+        for k, place in enumerate(places):
+            x[i * len(places) + k, place] = value
+    gamma, beta = parameters(cols, cuda_device, 22)
+    stats = torch.empty(len(x), 2, device=cuda_device)
+    y = ops.layer_norm(x, gamma, beta, out_dtype=torch.float32, stats=stats)
+    assert torch.equal(y[:-3], beta.repeat(len(x) - 3, 1)) and not stats[:-3, 1].any()
+    want = x[:-3].double().mean(1)
+    assert bool(((stats[:-3, 0].double() - want).abs() <= 64 * U * x[:-3].double().abs().amax(1)).all())
+    assert torch.isnan(y[-2]).all()
+    for row in (-3, -1):
+        assert torch.equal(y[row], ops.layer_norm(x[row:][:1].clone(), gamma, beta, out_dtype=torch.float32)[0]) and torch.isfinite(y[row]).all()
+
+
 @pytest.mark.parametrize("kind,p", [("none", 0.0), ("relu", 0.0), ("gelu_erf", 0.2), ("gelu_tanh", 0.0)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("cols,rows", [(1025, 2600), (2048, 1300), (2049, 1300), (4001, 700), (9000, 500), (16_384, 470), (16_386, 460), (24_576, 450), (24_577, 460), (33_538, 600),
