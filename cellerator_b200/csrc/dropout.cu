@@ -24,7 +24,8 @@ struct dropout_params {
 // with no division.  Q = 2 for two-byte elements in rows of whole 16-byte pieces, where a piece is one load and one store.
 // WHOLE: rows are whole pieces and every access is aligned.
 //
-// Bound by the integer pipe: ten rounds are 20 products of 32 x 32 bits and 20 xors for four values, whatever the type.  500,000 x 128
+// Bound by integer work: ten rounds are 20 products of 32 x 32 bits and 20 xors for four values, whatever the type; the ALU pipe is busy 54 % of
+// the cycles, the FMA pipe, which multiplies, 37 %, and warps wait for one of them or to be dispatched to it.  500,000 x 128
 // bf16 64 us (4.0 TB/s, 61 % of a copy; 68 with 8-byte pieces, 89 before loads and stores lost their branches); 48 million values of
 // fp32 70 us (84 %), of bf16 49 us (59 %).  The rounds' keys come out of the launch's constants: worked out by each thread, they were
 // 20 more additions.

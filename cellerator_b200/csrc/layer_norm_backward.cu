@@ -53,8 +53,8 @@ __device__ __forceinline__ void row_terms(float mean, float rstd, const float *g
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  Columns past the last hold
 // zeros in dy, so that they add nothing.  1,000,000 x 64, fp32 and a bf16 dy, GELU (tanh) and dropout: 169 us, 58 % of a copy, bound by
-// instructions (the random words and the slope; 175 us with one column at a time, 212 with an activation chosen per quad, 182 before the slope was rearranged);
-// without either 97 us.
+// instructions (the random words and the slope; 62 % of the issue slots, ALU and FMA pipes 44 %; 175 us with one column at a time, 212 with an activation chosen per quad, 182 before the slope was rearranged);
+// without either 101 us for 48 million values (87 %).
 template<int SX, int SG, bool HALVES, int ITEMS>
 __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? 3 : 2) layer_norm_back_narrow_kernel(const layer_norm_params p) {
     __shared__ float meet[kNarrowThreads / 32][ITEMS * 4 * 32];
@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(kNarrowThreads, ITEMS == 2 ? 3 : 2) layer_norm
 constexpr int kBlockQuads = 2, kBlockThreads = kBlockColumns / (4 * kBlockQuads); // of a thread; of a block, at most
 
 // A block per row; a thread keeps the sums of its columns from row to row.  gamma and beta are in shared memory: the sums, a row and
-// the next one's values take the registers.  48 million values of 4,000 columns: fp32 132 us (66 % of a copy), bf16 96 us (45 %), one
-// barrier a row; with GELU and dropout 183 and 149, bound by instructions.
+// the next one's values take the registers.  48 million values of 4,000 columns: fp32 132 us (66 % of a copy), bf16 97 us (45 %), one
+// barrier a row and half of the issue slots; with GELU and dropout 183 and 149, bound by instructions.
 template<int SX, int SG, bool HALVES>
 __global__ void __launch_bounds__(kBlockThreads) layer_norm_back_block_kernel(const layer_norm_params p) {
     constexpr int QT = kBlockQuads;

@@ -38,9 +38,10 @@ __device__ __forceinline__ void cut_off(float (&v)[4], int at, int n, float cent
 }
 
 // A group of p.lanes lanes per row; the next rows' values are on their way while these are worked on.  gamma and beta come out of
-// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 70 us, 5.6 TB/s,
-// 86 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
-// once).  GELU and dropout are bound by instructions: 48 million values 90 us.
+// shared memory: a lane's columns of them would take a third of its registers.  1,000,000 x 64 fp32 to bf16 with relu: 71 us, 5.5 TB/s,
+// 84 % of a copy, bound by HBM (74 us with a choice of activation and alignment for every quad, 86 with a row's loads waited for at
+// once).  GELU and dropout are bound by instructions, 63 % of the issue slots with the FMA pipe half full: 48 million values of 512 columns
+// 93 us.  So are 16-bit rows without either, 73 % of the slots: 43 us, 69 % of a copy.
 // Of fp32 rows a lane sums up distances from its first value, and the lanes' sums meet as distances from the first lane's: all of them zero in
 // a row of one value.  The sum of the values themselves is rounded, which such a row, if its value is large, shows as that rounding over
 // sqrt(epsilon).  Rows of 16-bit values need it not: the sum of 1,024 equal ones is a number of fp32.
@@ -183,8 +184,8 @@ struct block_statistics {
 
 // A block per row, the row in registers, its next row on the way where two fit and asked for in L2 where not; gamma and beta stay in
 // shared memory from row to row, as many columns of them as it holds (the rest of beta comes out of L2).
-// 4,099 x 33,538 bf16: 158 us, 53 % of a copy.  Half of the issue slots are taken (some 20 instructions a value; 41 with branches for each
-// quad, 277 us), and 30 warps, all at the same step of the same row, do not fill the others.  Measured against it: a cluster of eight blocks
+// 4,099 x 33,538 bf16: 160 us, 52 % of a copy.  Half of the issue slots are taken (54 %, some 22 instructions a value; 41 with branches for each
+// quad, 277 us), and 30 warps, all at the same step of the same row, wait for loads in the others (4.7 of them for each instruction).  Measured against it: a cluster of eight blocks
 // per row, whose threads kept gamma and beta of their columns, 373 us, waiting for its barriers; 512 threads with twice the quads 260;
 // the next row's quads loaded as soon as these are stored 173; two-wide products 183 (registers); the choices of activation and
 // dropout in the loop 180; three quads at a time 169; the columns walked twice as below 212.
@@ -297,7 +298,8 @@ cb200_status launch_rows(const layer_norm_params &p, int device, cudaStream_t st
 }
 
 // Rows that do not fit the registers: a block walks along its row twice, the second time out of L2.  40,000 columns, 48 million values:
-// fp32 97 us, bf16 68 us, bound by what L2 delivers (the row twice, gamma and beta: 116 and 94 with one column of these to a load);
+// fp32 96 us, bf16 67 us, bound by the wait for what L2 delivers (the row twice, gamma and beta; 7.8 warps an instruction; 116 and 94 with
+// one column of these to a load);
 // clusters of eight blocks that held a row took 183 and 122.
 constexpr int kLongThreads = 512, kLongQuads = 4; // quads that a thread has in flight
 

@@ -103,11 +103,13 @@ __device__ __forceinline__ void load4(const WT *p, float (&w)[4]) {
 // that of 32 / lanes classes of its entries, a row's that of its parts in order, and the product with B follows from shared memory.
 // Lanes past a part's end read its last entry again, and genes outside the matrix row 0 of A: both are staged as gene -1, whose row
 // counts as zeros whatever it holds.  Segments without such genes, up to the last whole piece of 8 entries a class, take the branch that
-// does not look.
+// does not look, where every lane holds columns: of ranks that are no power of two times a slice some lanes hold none, and all segments
+// take the branch that looks (4,099 x 33,538, bf16: rank 12 95 us where rank 16 takes 76; rank 24 94, rank 32 90).  Ranks that are no multiple
+// of half a 16-byte slice go column by column, and rank 50 twice along the row (525 us).
 //
 // 4,099 x 33,538, 8 bits, rank 16 bf16: 75 us, bound by what the SMs get out of L2 in pieces of 32 bytes at random places (a row of A, a
-// scale and a zero-point for each entry).  50,000 x 4,000, 4 bits, rank 32: 292 us, bound by L1's wavefronts (72 %, two for an entry) and
-// instructions (62 % of the slots, six for an entry in its share of a warp).  Before loads lost their branches 104 and 437.  Measured
+// scale and a zero-point for each entry; L1 and texture 70 %, issue 42 %).  50,000 x 4,000, 4 bits, rank 32: 292 us, bound by L1's wavefronts
+// (71 %, two for an entry) and instructions (66 % of the slots, six for an entry in its share of a warp).  Before loads lost their branches 104 and 437.  Measured
 // against it: scales and zero-points in shared memory, with fewer blocks an SM, 112 and 430 us; a third stage of loads under way 84; rows
 // of A kept in L1 79 and 298; scales and zero-points side by side, laid so in a launch before, 77 and 305; parts of 256 entries 86 and
 // 369; four blocks an SM by launch bounds 93, and with four rows of A in flight instead of eight 85 and
