@@ -719,7 +719,7 @@ cb200_status cb200_dropout_rows(const cb200_dropout_matrix *matrix, void *stream
  * var the mean of the squared differences.  epilogue: CB200_EPILOGUE_NONE, _RELU, _GELU_ERF or _GELU_TANH (beta is the
  * bias).  1 to 65,536 columns, fewer than 2^32 rows; more are refused.
  * Forward writes y (which may be x, as for dropout) and, when asked, stats.  GELU's factor of z is off by 4.5e-7 at most with the
- * erf form, 2e-7 with the tanh form (its slope by 2e-6): not the bits of the projection's epilogue of the same name.
+ * erf form, some 2e-7 with the tanh form (its slope 2e-6): not the bits of the projection's epilogue of the same name.
  * A row of one value has u = 0.  Squares and sums are fp32: a row whose variance passes its range (values that differ by 10^19)
  * has 1 / sigma = 0, which makes u 0 as well, and one whose sum does is NaN.
  * Backward reads x, dy and the stats of the forward call with the same parameters, epilogue and dropout, and writes
